@@ -41,7 +41,7 @@ typedef enum {
   LH_ERR_INVALID = -1,     /* bad argument (NULL, rank, shape mismatch)        */
   LH_ERR_UNSUPPORTED = -2, /* valid request this backend has no kernel for     */
   LH_ERR_CUDA = -3,        /* CUDA runtime / driver error                      */
-  LH_ERR_DEVICE = -4,      /* a kernel reported a bounded wait that ran out    */
+  LH_ERR_DEVICE = -4,      /* a kernel reported a bounded wait that ran out, or an index operand outside its table */
   LH_ERR_COMM = -5,        /* NCCL error or communicator not initialised       */
   LH_ERR_NOMEM = -6
 } lh_status_t;
@@ -247,6 +247,78 @@ int lh_b200_elementwise(lh_ctx_t* ctx, int kind, const lh_memref_t* out, const l
 int lh_b200_embedding(lh_ctx_t* ctx, const lh_memref_t* out, const lh_memref_t* ids, const lh_memref_t* wte,
                       const lh_memref_t* wpe, int period);
 
+/* ------------------------------------------------- a decoding step's operators */
+/*
+ * A paged key-value cache: k_pages and v_pages are (pages, page_size, Hkv, D) views of one
+ * pool (any strides, unit in D; a (pages, Hkv, page_size, D) pool is the permuted view), a
+ * page of which belongs to one sequence at a time (or, read only, to several that share a
+ * prefix). The reference decodes nothing and has no counterpart: its attention is over
+ * contiguous K and V (examples/llama/ref_model.py:114-166), which is what a cache's contents
+ * stand for.
+ *
+ * Index operands live on the device and are checked there: an entry that points outside its
+ * table is skipped, everything else is done, and the next lh_b200_sync returns LH_ERR_DEVICE.
+ */
+
+/*
+ * Rows of new tokens enter the cache. For token t, with slot s = slots[t] (page s / page_size,
+ * row s % page_size of it) and theta > 0:
+ *   q[t] <- rot(q[t], positions[t])  in place (q may be NULL)
+ *   k_pages[s] <- rot(k[t], positions[t]);  v_pages[s] <- v[t]
+ * rot is lh_b200_rope's rotation of pairs (2i, 2i+1), with a position for every token and the
+ * angle reduced in f64, so that it holds at any distance; values are rotated in f32 and rounded
+ * once to the type they are stored in. theta == 0: no rotation, q is left alone, positions may
+ * be NULL. A negative slot marks a row of padding: its k and v go nowhere (its q is rotated).
+ * Slots of one call must differ; where two are equal that slot holds a mixture of both rows.
+ * q (T, Hq, D), k, v (T, Hkv, D) of one type (f32, bf16, f16), pages of one type (the same or
+ * another), D even to rotate and at most 512; slots, positions (T) i32 or i64.
+ */
+int lh_b200_paged_append(lh_ctx_t* ctx, const lh_memref_t* q, const lh_memref_t* k, const lh_memref_t* v,
+                         const lh_memref_t* k_pages, const lh_memref_t* v_pages, const lh_memref_t* slots,
+                         const lh_memref_t* positions, float theta);
+
+/*
+ * Attention of S new tokens (one, or a few proposed ones) over the cache: per sequence b
+ *   o = softmax(scale . q K^T) V,   key j is row j % page_size of page page_table[b][j / page_size]
+ * over the first lengths[b] keys, the new tokens' own included; token s of S sees the first
+ * lengths[b] - S + s + 1 of them. A row that sees none is zeros. q, o (B, Hq, S, D), head h
+ * reads kv head h / (Hq / Hkv) as in lh_b200_attention_fwd; page_table (B, columns) and lengths
+ * (B) i32, columns past a sequence's last page are not read. q and the pages have one type (f32,
+ * bf16 or f16; o may have another), D at most 256. Scores, softmax and sums in f32; for 16-bit
+ * types P is rounded to the type before P V, as in lh_b200_attention_fwd. The work is cut by the
+ * lengths on the device, so a captured call follows them from replay to replay; the cut
+ * fixes the order of every sum, so a call repeats bit for bit.
+ * workspace: contiguous, 256-byte aligned, at least lh_b200_paged_attention_workspace bytes
+ * (LH_ERR_NOMEM below that); calls that can overlap on the GPU need one each. In a module the
+ * operand may be absent: the context's scratch is used.
+ */
+int lh_b200_paged_attention(lh_ctx_t* ctx, const lh_memref_t* o, const lh_memref_t* q, const lh_memref_t* k_pages,
+                            const lh_memref_t* v_pages, const lh_memref_t* page_table, const lh_memref_t* lengths,
+                            const lh_memref_t* workspace, float scale);
+int lh_b200_paged_attention_workspace(lh_ctx_t* ctx, const lh_memref_t* q, const lh_memref_t* k_pages, size_t* bytes);
+
+/*
+ * Draws one token per row of logits (rows, vocabulary). With x a row, M its maximum and
+ * weights w_i = exp((x_i - M) / temperature):
+ *   top_k  keeps the k largest x (equal ones: lowest index first); k <= 0 or >= vocabulary: all
+ *   top_p  keeps, of those, from the largest down, as many as it takes for their sum to reach
+ *          top_p times the sum of what top_k left, at least one; top_p >= 1: all
+ *   min_p  keeps, of those, the ones with w_i >= min_p; the largest always stays
+ *   tokens[r] = the lowest kept index whose running sum, in index order, is above
+ *          uniform[r] times the kept sum;   logprobs[r] = log(w / kept sum) of it
+ * temperature <= 0 takes the first of the largest (log-probability 0). NaN and -inf are never
+ * drawn; a row of nothing else gives token -1 and log-probability -inf; tokens at +inf share
+ * the weight equally. A setting that is NaN is off (temperature: greedy); a random number
+ * outside [0, 1) takes the first or the last kept token. Weights are exact to 2^-42 of the
+ * largest and summed as whole numbers: the draw does not depend on how a row is split.
+ * logits f32, bf16 or f16 with unit stride along the vocabulary (at most 2^20); tokens, top_k
+ * (rows) i32 or i64; uniform, temperature, top_p, min_p, logprobs (rows) f32; all of
+ * temperature (1), top_k, top_p, min_p and logprobs may be NULL. No counterpart in the reference.
+ */
+int lh_b200_sample(lh_ctx_t* ctx, const lh_memref_t* tokens, const lh_memref_t* logprobs, const lh_memref_t* logits,
+                   const lh_memref_t* uniform, const lh_memref_t* temperature, const lh_memref_t* top_k,
+                   const lh_memref_t* top_p, const lh_memref_t* min_p);
+
 /* ------------------------------------------------------------- collectives */
 /* Tensor-parallel plumbing: the reference's only precedent is the MPI
  * weight-stationary example (examples/mpi/feed-forward-mpi.py:213-228). NCCL is
@@ -349,7 +421,10 @@ typedef enum {
   LH_OP_EVENT_WAIT = 14,
   LH_OP_RESERVE_SMS = 15,
   LH_OP_REDUCE_NORM_GATHER = 16,
-  LH_OP_GEMM_ROPE = 17
+  LH_OP_GEMM_ROPE = 17,
+  LH_OP_PAGED_APPEND = 18,
+  LH_OP_PAGED_ATTENTION = 19,
+  LH_OP_SAMPLE = 20
 } lh_op_kind_t;
 
 /* An operand: a view into a slot. slot < 0 means "absent". */
@@ -382,6 +457,9 @@ typedef struct {
  *   REDUCE_NORM_GATHER xn, part, h, weight      f0 = eps
  *   GEMM_ROPE   d, a, b                         i0 = rotary columns, i1 = head size, i2 = sequence
  *                                               length, f0 = theta, f1 = first position
+ *   PAGED_APPEND q, k, v, k_pages, v_pages, slots, positions          f0 = theta
+ *   PAGED_ATTENTION o, q, k_pages, v_pages, page_table, lengths, workspace    f0 = scale
+ *   SAMPLE      tokens, logprobs, logits, uniform, temperature, top_k, top_p, min_p
  */
 typedef struct {
   int32_t kind;

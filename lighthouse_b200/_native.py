@@ -74,7 +74,10 @@ EW_COPY, EW_ADD, EW_MUL, EW_ACT, EW_ADD_ACT, EW_SILU_MUL, EW_SCALE, EW_FILL, EW_
     OP_RESERVE_SMS,
     OP_REDUCE_NORM_GATHER,
     OP_GEMM_ROPE,
-) = range(1, 18)
+    OP_PAGED_APPEND,
+    OP_PAGED_ATTENTION,
+    OP_SAMPLE,
+) = range(1, 21)
 
 
 class MemRef(Structure):
@@ -154,6 +157,10 @@ _PROTOTYPES = {
     "lh_b200_rope": (c_int, [c_void_p, POINTER(MemRef), c_float, c_int]),
     "lh_b200_elementwise": (c_int, [c_void_p, c_int] + [POINTER(MemRef)] * 3 + [c_int, c_float]),
     "lh_b200_embedding": (c_int, [c_void_p] + [POINTER(MemRef)] * 4 + [c_int]),
+    "lh_b200_paged_append": (c_int, [c_void_p] + [POINTER(MemRef)] * 7 + [c_float]),
+    "lh_b200_paged_attention": (c_int, [c_void_p] + [POINTER(MemRef)] * 7 + [c_float]),
+    "lh_b200_paged_attention_workspace": (c_int, [c_void_p, POINTER(MemRef), POINTER(MemRef), POINTER(c_size_t)]),
+    "lh_b200_sample": (c_int, [c_void_p] + [POINTER(MemRef)] * 8),
     "lh_b200_comm_unique_id": (c_int, [c_char_p, c_void_p]),
     "lh_b200_comm_init": (c_int, [c_void_p, c_char_p, c_void_p, c_int, c_int]),
     "lh_b200_comm_destroy": (c_int, [c_void_p]),

@@ -188,6 +188,67 @@ class CudaContext:
         mo, mi, mw, mp = (as_memref(t) for t in (out, ids, wte, wpe))
         N.check(self._lib.lh_b200_embedding(self.handle, _ref(mo), _ref(mi), _ref(mw), _ref(mp), int(period)), self.handle, "lh_b200_embedding")
 
+    # -- a decoding step's operators (see include/lh_b200.h for semantics) -------------------
+    def _on_device(self, *operands) -> None:
+        for t in operands:
+            if t is not None and not isinstance(t, N.MemRef) and t.is_cuda and t.device.index != self.device:
+                raise ValueError(f"an operand is on {t.device}, the context on cuda:{self.device}")
+
+    def paged_append(self, q, k, v, k_pages, v_pages, slots, positions=None, theta: float = 10000.0) -> None:
+        """New tokens' rows enter the paged cache: q (T, Hq, D), rotated in place, may be None;
+        k, v (T, Hkv, D); pages (pages, page_size, Hkv, D); slots, positions (T) i32 or i64, a
+        negative slot is padding. ``theta`` 0: no rotation."""
+        self._on_device(q, k, v, k_pages, v_pages, slots, positions)
+        m = [as_memref(t) for t in (q, k, v, k_pages, v_pages, slots, positions)]
+        N.check(self._lib.lh_b200_paged_append(self.handle, *map(_ref, m), float(theta)), self.handle, "lh_b200_paged_append")
+
+    def paged_attention_workspace(self, q, k_pages) -> int:
+        """Bytes of workspace that ``paged_attention`` needs for operands of these shapes."""
+        n = ctypes.c_size_t()
+        mq, mk = as_memref(q), as_memref(k_pages)
+        N.check(self._lib.lh_b200_paged_attention_workspace(self.handle, _ref(mq), _ref(mk), byref(n)), self.handle, "lh_b200_paged_attention_workspace")
+        return n.value
+
+    def paged_attention(self, o, q, k_pages, v_pages, page_table, lengths, scale: float, workspace=None) -> None:
+        """Attention of new tokens over the paged cache: q, o (B, Hq, S, D); pages (pages,
+        page_size, Hkv, D); page_table (B, columns), lengths (B) i32. ``workspace``: a CUDA
+        tensor of ``paged_attention_workspace`` bytes; without one the context keeps one for each
+        stream it launches on, and gives each call inside a CUDA graph capture one of its own."""
+        self._on_device(o, q, k_pages, v_pages, page_table, lengths, workspace)
+        m = [as_memref(t) for t in (o, q, k_pages, v_pages, page_table, lengths)]
+        if workspace is None:
+            workspace = self._workspace(m[1], m[2])
+        if isinstance(workspace, N.MemRef):
+            mw = workspace
+        else:  # bytes, whatever the element type
+            if not workspace.is_cuda or not workspace.is_contiguous():
+                raise ValueError("the workspace must be a contiguous CUDA tensor")
+            mw = N.memref(workspace.data_ptr(), (workspace.numel() * workspace.element_size() // 4,), (1,), N.LH_F32)
+        N.check(self._lib.lh_b200_paged_attention(self.handle, *map(_ref, m), _ref(mw), float(scale)), self.handle, "lh_b200_paged_attention")
+
+    def _workspace(self, mq, mk):
+        torch = _torch()
+        need = self.paged_attention_workspace(mq, mk)
+        kept = self.__dict__.setdefault("_workspaces", {})
+        stream = self.stream_handle()
+        ws = kept.get(stream)
+        capturing = torch.cuda.is_current_stream_capturing()
+        if ws is None or ws.numel() < need or capturing:
+            ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{self.device}")
+            # none is given back while the context lives: work still queued, or a captured graph,
+            # may use it
+            self.__dict__.setdefault("_workspaces_held", []).append(ws)
+            if not capturing:
+                kept[stream] = ws
+        return ws
+
+    def sample(self, tokens, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, logprobs=None) -> None:
+        """One token per row of logits (rows, vocabulary), drawn with ``uniform`` (rows) in [0, 1)
+        from what top-k, then top-p, then min-p leave; settings are (rows) tensors or None."""
+        self._on_device(tokens, logits, uniform, temperature, top_k, top_p, min_p, logprobs)
+        m = [as_memref(t) for t in (tokens, logprobs, logits, uniform, temperature, top_k, top_p, min_p)]
+        N.check(self._lib.lh_b200_sample(self.handle, *map(_ref, m)), self.handle, "lh_b200_sample")
+
     # -- collectives ---------------------------------------------------------------
     def comm_init(self, unique_id: bytes, rank: int, world: int, nccl_path: str | None = None) -> None:
         buf = ctypes.create_string_buffer(unique_id, 128)

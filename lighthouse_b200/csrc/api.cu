@@ -7,6 +7,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace lh {
 
@@ -247,6 +248,7 @@ extern "C" int lh_b200_sync(lh_ctx_t* ctx) {
     for (const AttnSplitPlan& pl : ctx->attn_plans)
       if (pl.counters) cudaMemsetAsync(pl.counters, 0, static_cast<size_t>(pl.n_slots) * 2 * sizeof(int), ctx->stream);
     cudaStreamSynchronize(ctx->stream);
+    if (st == DEV_BAD_INDEX) return set_error(ctx, LH_ERR_DEVICE, "a page, slot or length operand points outside its table; those entries were skipped (device status %d)", st);
     return set_error(ctx, LH_ERR_DEVICE, "a kernel gave up on a bounded wait (device status %d)", st);
   }
   return LH_OK;
@@ -679,6 +681,18 @@ size_t op_scratch_bytes(lh_ctx* ctx, const lh_op_t& op) {
     }
     return static_cast<size_t>(q.shape[q.rank - 2]) * static_cast<size_t>(k.shape[k.rank - 2]) * sizeof(float);
   }
+  if (op.kind == LH_OP_PAGED_ATTENTION && op.operands[6].slot < 0 && op.operands[1].slot >= 0 && op.operands[2].slot >= 0) {
+    auto shape_of = [](const lh_view_t& v) {
+      lh_memref_t m;
+      memset(&m, 0, sizeof(m));
+      m.rank = v.rank; m.dtype = v.dtype;
+      for (int i = 0; i < LH_MAX_RANK; ++i) m.shape[i] = v.shape[i];
+      return m;
+    };
+    const lh_memref_t q = shape_of(op.operands[1]), k = shape_of(op.operands[2]);
+    size_t need = 0;
+    return lh_b200_paged_attention_workspace(ctx, &q, &k, &need) ? 0 : need;
+  }
   if (op.kind == LH_OP_GEMM) {
     const lh_view_t& a = op.operands[1];
     const lh_view_t& b = op.operands[2];
@@ -713,7 +727,7 @@ extern "C" int lh_b200_module_create(lh_ctx_t* ctx, const char* entry_name, cons
   *out = nullptr;
   const int nslots = nargs + ntemps;
   for (int i = 0; i < nops; ++i) {
-    if (ops[i].kind < LH_OP_GEMM || ops[i].kind > LH_OP_GEMM_ROPE) return set_error(ctx, LH_ERR_INVALID, "module_create: op %d has unknown kind %d", i, ops[i].kind);
+    if (ops[i].kind < LH_OP_GEMM || ops[i].kind > LH_OP_SAMPLE) return set_error(ctx, LH_ERR_INVALID, "module_create: op %d has unknown kind %d", i, ops[i].kind);
     for (int j = 0; j < LH_MAX_OPERANDS; ++j) {
       const lh_view_t& v = ops[i].operands[j];
       if (v.slot >= nslots) return set_error(ctx, LH_ERR_INVALID, "module_create: op %d operand %d names slot %d of %d", i, j, v.slot, nslots);
@@ -808,6 +822,25 @@ static int run_ops(lh_module* m, void* const* arg_ptrs) {
       case LH_OP_RESERVE_SMS: rc = lh_b200_reserve_sms(ctx, op.i0); break;
       case LH_OP_REDUCE_NORM_GATHER: rc = lh_b200_reduce_norm_gather(ctx, o[0], o[1], o[2], o[3], op.f0); break;
       case LH_OP_ALLGATHER: rc = lh_b200_allgather(ctx, o[0], o[1]); break;
+      case LH_OP_PAGED_APPEND: rc = lh_b200_paged_append(ctx, o[0], o[1], o[2], o[3], o[4], o[5], o[6], op.f0); break;
+      case LH_OP_PAGED_ATTENTION: {
+        // without a workspace of its own the operator uses the context's scratch, like the
+        // other operators that need some (sized when the module was created)
+        lh_memref_t ws;
+        if (!o[6] && o[1] && o[2]) {
+          size_t need = 0;
+          rc = lh_b200_paged_attention_workspace(ctx, o[1], o[2], &need);
+          if (!rc) rc = ensure_scratch(ctx, need);
+          if (rc) break;
+          memset(&ws, 0, sizeof(ws));
+          ws.allocated = ws.aligned = ctx->scratch;
+          ws.rank = 1; ws.dtype = LH_F32; ws.shape[0] = static_cast<int64_t>(need / sizeof(float)); ws.strides[0] = 1;
+          o[6] = &ws;
+        }
+        rc = lh_b200_paged_attention(ctx, o[0], o[1], o[2], o[3], o[4], o[5], o[6], op.f0);
+        break;
+      }
+      case LH_OP_SAMPLE: rc = lh_b200_sample(ctx, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]); break;
       case LH_OP_GEMM_ROPE: rc = lh_b200_gemm_rope(ctx, o[0], o[1], o[2], op.i0, op.i1, op.i2, op.f0, static_cast<int>(op.f1)); break;
       default: rc = set_error(ctx, LH_ERR_INVALID, "unknown op kind %d", op.kind);
     }

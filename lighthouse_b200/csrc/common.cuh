@@ -131,6 +131,18 @@ inline int64_t numel(const lh_memref_t* m) {
   return n;
 }
 
+// Makes the context's device current while a call launches, whatever device the caller has
+// current, and puts the caller's back.
+struct DeviceScope {
+  int prev = -1;
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&prev) != cudaSuccess || prev == device || cudaSetDevice(device) != cudaSuccess) prev = -1;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
 // ------------------------------------------------------------- GEMM problem
 // One (possibly batched) product with its epilogue, in element strides.
 struct GemmProblem {

@@ -161,6 +161,7 @@ class PlanOp:
             q, k = self.operands[1], self.operands[2]
             f = 4 * math.prod(q.shape[:-2]) * q.shape[-2] * k.shape[-2] * q.shape[-1]
             return f // 2 if self.attrs.get("causal") else f
+        # paged_attention: the keys are counted by the lengths on the device
         return 0
 
 
@@ -182,6 +183,9 @@ _KIND_CODES = {
     "reserve_sms": N.OP_RESERVE_SMS,
     "reduce_norm_gather": N.OP_REDUCE_NORM_GATHER,
     "gemm_rope": N.OP_GEMM_ROPE,
+    "paged_append": N.OP_PAGED_APPEND,
+    "paged_attention": N.OP_PAGED_ATTENTION,
+    "sample": N.OP_SAMPLE,
 }
 
 
@@ -245,6 +249,21 @@ class Plan:
     def embedding(self, out, ids, wte, wpe=None, period: int = 0):
         self.ops.append(PlanOp("embedding", [out, ids, wte, wpe], {"period": int(period)}))
         return out
+
+    def paged_append(self, q, k, v, k_pages, v_pages, slots, positions=None, theta: float = 10000.0):
+        """New tokens' rows enter the paged cache; q and k rotated to ``positions`` (q in place)."""
+        self.ops.append(PlanOp("paged_append", [q, k, v, k_pages, v_pages, slots, positions], {"theta": float(theta)}))
+        return k_pages
+
+    def paged_attention(self, o, q, k_pages, v_pages, page_table, lengths, scale: float, workspace=None):
+        """Attention of the new tokens over the paged cache (the context's scratch without ``workspace``)."""
+        self.ops.append(PlanOp("paged_attention", [o, q, k_pages, v_pages, page_table, lengths, workspace], {"scale": float(scale)}))
+        return o
+
+    def sample(self, tokens, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, logprobs=None):
+        """One token per row of logits, drawn with the given random numbers."""
+        self.ops.append(PlanOp("sample", [tokens, logprobs, logits, uniform, temperature, top_k, top_p, min_p]))
+        return tokens
 
     def allreduce(self, buf):
         """Sum over the tensor-parallel ranks, in place."""
@@ -317,6 +336,10 @@ class Plan:
             at = op.attrs
             if op.kind == "gemm":
                 o.i0, o.i1 = ACT_CODES[at.get("act", "none")], int(at.get("flags", 0)) | ((int(at.get("tile_n", 0)) // 8) << 8)
+            elif op.kind == "paged_append":
+                o.f0 = at["theta"]
+            elif op.kind == "paged_attention":
+                o.f0 = at["scale"]
             elif op.kind == "attention":
                 o.f0, o.i0 = at["scale"], int(at.get("causal", False))
             elif op.kind in ("layernorm", "rmsnorm", "reduce_norm_gather"):
