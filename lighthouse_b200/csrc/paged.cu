@@ -489,6 +489,22 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const PagedPar
   }
 }
 
+int join_launch(lh_ctx* ctx, const PagedParams& p, int ctas) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(p.rows < p.unit_rows ? p.rows : p.unit_rows));
+  cfg.blockDim = dim3(JOIN_THREADS);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LH_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, paged_join_kernel, p));
+  LH_CHECK_LAUNCH(ctx, "paged_join_kernel");
+  return LH_OK;
+}
+
 typedef void (*PagedKernel)(const PagedParams);
 template <typename T>
 PagedKernel simt_kernel_for(int D, bool vec) {
@@ -642,8 +658,9 @@ extern "C" int lh_b200_paged_attention_workspace(lh_ctx_t* ctx, const lh_memref_
   const int Dp = static_cast<int>((q->shape[3] + 3) / 4 * 4);
   const int64_t rows = q->shape[1] / k_pages->shape[2] * q->shape[2];
   const size_t simt = workspace_for(simt_ctas(ctx), SIMT_ROWS, Dp).bytes;
-  *bytes = simt;
-  (void)rows;
+  const int D = q->shape[3] > 256 ? 256 : static_cast<int>(q->shape[3]);
+  const size_t mma = workspace_for(paged_mma_ctas(ctx, D), paged_mma_unit_rows(rows, D), Dp).bytes;
+  *bytes = simt > mma ? simt : mma;
   return LH_OK;
 }
 
@@ -681,9 +698,10 @@ extern "C" int lh_b200_paged_attention(lh_ctx_t* ctx, const lh_memref_t* o, cons
   p.scale_log2 = scale * 1.4426950408889634f;
   p.Dp = (p.D + 3) / 4 * 4;
   p.dev_status = ctx->dev_status;
-  p.unit_rows = SIMT_ROWS;
+  const bool mma = paged_mma_supported(k_pages, v_pages);
+  p.unit_rows = mma ? paged_mma_unit_rows(p.rows, p.D) : SIMT_ROWS;
   p.tile = SIMT_TILE;
-  int64_t ctas = simt_ctas(ctx);
+  const int ctas = static_cast<int>(mma ? paged_mma_ctas(ctx, p.D) : simt_ctas(ctx));
   p.row_groups = (p.rows + p.unit_rows - 1) / p.unit_rows;
   if (static_cast<int64_t>(p.Hkv) * p.row_groups > 0x7fffffffll) return set_error(ctx, LH_ERR_UNSUPPORTED, "paged_attention: too many query rows");
   const Workspace w = workspace_for(ctas, p.unit_rows, p.Dp);
@@ -693,21 +711,14 @@ extern "C" int lh_b200_paged_attention(lh_ctx_t* ctx, const lh_memref_t* o, cons
   p.ml = reinterpret_cast<float2*>(base + w.ml);
   p.part = reinterpret_cast<float*>(base + w.part);
   DeviceScope scope(ctx->device);
+  if (mma) {
+    rc = paged_mma_launch(ctx, p, q->dtype, ctas);
+    if (rc) return rc;
+    return join_launch(ctx, p, ctas);
+  }
   const bool vec = p.D % 4 == 0 && aligned_view(k_pages, 4) && aligned_view(v_pages, 4);
   PagedKernel kernel = q->dtype == LH_F32 ? simt_kernel_for<float>(p.D, vec) : q->dtype == LH_BF16 ? simt_kernel_for<__nv_bfloat16>(p.D, vec) : simt_kernel_for<__half>(p.D, vec);
   kernel<<<static_cast<unsigned>(ctas), SIMT_THREADS, 0, ctx->stream>>>(p);
   LH_CHECK_LAUNCH(ctx, "paged_simt_kernel");
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(p.rows < p.unit_rows ? p.rows : p.unit_rows));
-  cfg.blockDim = dim3(JOIN_THREADS);
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  LH_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, paged_join_kernel, p));
-  LH_CHECK_LAUNCH(ctx, "paged_join_kernel");
-  return LH_OK;
+  return join_launch(ctx, p, ctas);
 }

@@ -149,9 +149,10 @@ __device__ __forceinline__ float exp2_safe(float x, float m) { return m == -INFI
 __device__ __forceinline__ int row_token(const PagedParams& p, int row) { return row / p.group; }
 __device__ __forceinline__ int row_head(const PagedParams& p, int hkv, int row) { return hkv * p.group + row % p.group; }
 
-int paged_mma_supported(const lh_memref_t* q, const lh_memref_t* k, const lh_memref_t* v);
-int paged_mma_unit_rows(int rows, int D);
-int paged_mma_ctas(const lh_ctx* ctx, int rows, int D);
+// The tensor-core kernel (paged_mma.cu).
+bool paged_mma_supported(const lh_memref_t* k, const lh_memref_t* v);
+int paged_mma_unit_rows(int64_t rows, int D);
+int paged_mma_ctas(const lh_ctx* ctx, int D);
 int paged_mma_launch(lh_ctx* ctx, PagedParams& p, int dtype, int ctas);
 
 }  // namespace lh

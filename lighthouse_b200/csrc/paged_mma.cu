@@ -1,0 +1,446 @@
+// Attention of new tokens over a paged cache of 16-bit rows (16-byte aligned), the kernel that
+// serving runs. Per key and kv head it reads 4 D bytes and computes 4 D flop per query row, so
+// with the handful of rows that share a kv head it is bound by the cache's bytes from HBM: at
+// 6.5 TB/s one SM gets a key of D = 128 every 21 clocks, and everything else only has to fit
+// under that. mma.sync does: the products of 16 keys are 16 instructions for up to eight rows
+// (tcgen05's 128-row tiles would be filled to a sixteenth, and its operands would have to be
+// laid out by one more pass through shared memory for no byte less from HBM).
+//
+// Both products are taken transposed, S^T = K Q^T and O^T += V^T P^T, so that the long sides (16
+// keys, then 16 head dimensions) fill the instruction's m16 and the query rows its n8: eight rows
+// cost half of what they would as a half-empty m16, accumulators included. S^T leaves the
+// first product with keys along the rows; movmatrix turns its 8 x 8 blocks into the second
+// product's operand in registers.
+//
+// Each warp runs by itself: it takes 16 of the tile's 64 keys, fetches them with cp.async into
+// its own ring of stages and keeps its own online softmax, so the main loop has no block-wide
+// barrier. The four warps are joined when the CTA leaves a unit; the ring is already being
+// filled for the next unit meanwhile.
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace lh {
+namespace {
+
+constexpr int THREADS = 128;
+constexpr int TILE = 64;  // keys of a tile, 16 per warp
+constexpr int SUB = 16;
+
+template <int DP>
+struct Shape {
+  static constexpr int stage_bytes = 2 * SUB * DP * 2;  // K and V rows of one warp's 16 keys
+  static constexpr int stages = DP == 64 ? 6 : 3;
+  static constexpr int ctas_per_sm = DP == 256 ? 1 : 2;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float bits_to_f32(uint32_t bits16) {
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
+  else return __uint_as_float(bits16 << 16);
+}
+
+// What the ring's producer side knows: the next tile to fetch and, one step ahead of its use,
+// the page that holds this lane's key of it.
+struct Fetch {
+  TileCursor at;
+  int64_t left;  // tiles still to fetch
+  int page_id;
+};
+
+template <typename T, int DP, int NT, bool WHOLE_PAGE>
+__global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_kernel(const PagedParams p) {
+  constexpr int STAGES = Shape<DP>::stages, STAGE_BYTES = Shape<DP>::stage_bytes, V_OFF = STAGE_BYTES / 2;
+  constexpr int CHUNKS = DP / 8;             // 16-byte chunks of a row
+  constexpr int ROWS_AT_ONCE = 32 / CHUNKS;  // rows that one cp.async per lane covers
+  constexpr int KSTEPS = DP / 16;
+  constexpr int OB = DP + 4;  // row pitch of the join buffer: its 8 x 4 lanes hit 32 banks
+  extern __shared__ __align__(128) char smem[];
+  __shared__ float wm[4][NT * 8], wl[4][NT * 8];
+  __shared__ uint32_t there[4][STAGES];  // which of a stage's 16 keys exist
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  grid_dependency_trigger();
+  int64_t lo, hi;
+  TileCursor at;
+  if (!find_stretch<THREADS>(p, lo, hi, at)) return;
+
+  const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE_BYTES;
+  char* const ring_ptr = smem + warp * STAGES * STAGE_BYTES;
+  float* const obuf = reinterpret_cast<float*>(smem + 4 * STAGES * STAGE_BYTES);
+  const T* const K = static_cast<const T*>(p.k);
+  const T* const V = static_cast<const T*>(p.v);
+
+  // ---- producer
+  const int chunk = lane % CHUNKS, row_in = lane / CHUNKS;
+  const bool chunk_there = chunk * 8 < p.D;
+  Fetch f;
+  f.at = at;
+  f.left = hi - lo;
+  // -1: no such key; INT_MIN would do as well, any id outside the pool is not fetched
+  auto look_up = [&]() {
+    const int j = f.at.t * TILE + warp * SUB + (WHOLE_PAGE ? 0 : lane & 15);
+    f.page_id = f.left > 0 && j < f.at.len ? p.table[f.at.b * p.stb + page_of(p, j) * p.stp] : -1;
+  };
+  look_up();
+  auto fetch = [&](int stage) {
+    if (f.left <= 0) return;
+    const int key0 = f.at.t * TILE + warp * SUB;
+    const int hkv = f.at.u / p.row_groups;
+    const bool inside = f.page_id >= 0 && f.page_id < p.num_pages;
+    const uint32_t base = ring + stage * STAGE_BYTES;
+    uint32_t mask;
+    if constexpr (WHOLE_PAGE) {
+      const int n = f.at.len - key0;
+      mask = !inside ? 0u : n >= SUB ? 0xffffu : (1u << n) - 1u;
+      if (n > 0 && !inside && lane == 0) report_bad_index(p.dev_status);
+      if (mask) {
+        const int slot = key0 - page_of(p, key0) * p.page;
+        const T* ks = K + f.page_id * p.skp + slot * p.sks + hkv * p.skh + chunk * 8;
+        const T* vs = V + f.page_id * p.svp + slot * p.svs + hkv * p.svh + chunk * 8;
+#pragma unroll
+        for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
+          const int row = i * ROWS_AT_ONCE + row_in;
+          const bool get = chunk_there && (mask >> row & 1);
+          const uint32_t dst = base + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
+          cp_async16(dst, get ? ks + row * p.sks : K, get ? 16 : 0);
+          cp_async16(dst + V_OFF, get ? vs + row * p.svs : V, get ? 16 : 0);
+        }
+      }
+    } else {
+      const int j = key0 + (lane & 15);
+      const bool live = j < f.at.len;
+      if (live && !inside) report_bad_index(p.dev_status);
+      mask = __ballot_sync(0xffffffffu, live && inside) & 0xffffu;
+      const int slot = j - page_of(p, j) * p.page;
+      const int64_t ko = live && inside ? f.page_id * p.skp + slot * p.sks + hkv * p.skh : 0;
+      const int64_t vo = live && inside ? f.page_id * p.svp + slot * p.svs + hkv * p.svh : 0;
+      if (mask) {
+#pragma unroll
+        for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
+          const int row = i * ROWS_AT_ONCE + row_in;
+          const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
+          const bool get = chunk_there && (mask >> row & 1);
+          const uint32_t dst = base + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
+          cp_async16(dst, get ? K + kr + chunk * 8 : K, get ? 16 : 0);
+          cp_async16(dst + V_OFF, get ? V + vr + chunk * 8 : V, get ? 16 : 0);
+        }
+      }
+    }
+    if (lane == 0) there[warp][stage] = mask;
+    --f.left;
+    if (++f.at.t == f.at.tiles && f.left > 0) f.at.next_unit(p);
+    look_up();
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) {
+    fetch(s);
+    cp_async_commit();
+  }
+
+  // ---- consumer
+  // ldmatrix addresses inside a stage: lane l gives row (l & 7) of matrix l / 8
+  const int mi = lane >> 3, r8 = lane & 7;
+  const int krow = (mi & 1) * 8 + r8, kchunk = mi >> 1;  // K: matrices (keys lo, k lo), (keys hi, k lo), (keys lo, k hi), (keys hi, k hi)
+  const int vrow = (mi >> 1) * 8 + r8, vchunk = mi & 1;  // V, transposed: (dims lo, keys lo), (dims hi, keys lo), (dims lo, keys hi), (dims hi, keys hi)
+  uint32_t qf[NT][KSTEPS][2];
+  float acc[NT][KSTEPS][4];
+  float m[NT][2], l[NT][2];  // query rows 2 t4 and 2 t4 + 1 of each n tile
+  int seen[NT][2];
+  int t0 = at.t, stage = 0;
+  bool fresh = true;
+  for (int64_t left = hi - lo; left > 0; --left) {
+    const int hkv = at.u / p.row_groups, row0 = (at.u % p.row_groups) * (NT * 8);
+    const int nrows = min(NT * 8, p.rows - row0);
+    if (fresh) {
+      fresh = false;
+      t0 = at.t;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int r = n * 8 + g, row = row0 + r;
+        const T* q = static_cast<const T*>(p.q) + at.b * p.sqb + (r < nrows ? row_head(p, hkv, row) * p.sqh + row_token(p, row) * p.sqs : 0);
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int d = k * 16 + i * 8 + t4 * 2;
+            const unsigned short* q16 = reinterpret_cast<const unsigned short*>(q) + d;
+            const uint32_t a = r < nrows && d < p.D ? q16[0] : 0u, b = r < nrows && d + 1 < p.D ? q16[1] : 0u;
+            qf[n][k][i] = a | b << 16;
+          }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          m[n][i] = -INFINITY;
+          l[n][i] = 0.f;
+          const int mine = row0 + n * 8 + t4 * 2 + i;
+          seen[n][i] = at.len - p.Sq + 1 + row_token(p, mine);
+        }
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[n][k][i] = 0.f;
+      }
+    }
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const uint32_t mask = there[warp][stage];
+    if (mask) {
+      const uint32_t base = ring + stage * STAGE_BYTES;
+      const int key0 = at.t * TILE + warp * SUB;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) {
+        uint32_t a[4];
+        ldmatrix4(a, base + krow * (DP * 2) + (((k * 2 + kchunk) ^ (krow & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<T>(s[n], a, qf[n][k][0], qf[n][k][1]);
+      }
+      const bool some_masked = key0 + SUB > at.len - p.Sq + 1;  // some row does not see some of these keys (or they do not exist)
+      const bool whole = mask == 0xffffu && !some_masked;
+      bool grows = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[n][i] *= p.scale_log2;
+          if (!whole) {
+            const int key = g + (i >> 1) * 8;
+            if (!(mask >> key & 1) || key0 + key >= seen[n][i & 1]) s[n][i] = -INFINITY;
+          }
+        }
+        grows |= fmaxf(s[n][0], s[n][2]) > m[n][0] || fmaxf(s[n][1], s[n][3]) > m[n][1];
+      }
+      // the running maximum is only brought up to date when some key passes it
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(s[n][i], s[n][i + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(top, m[n][i]);
+            const float alpha = top == -INFINITY ? 1.f : ex2(m[n][i] - top);
+            m[n][i] = top;
+            l[n][i] *= alpha;
+#pragma unroll
+            for (int k = 0; k < KSTEPS; ++k) {
+              acc[n][k][i] *= alpha;
+              acc[n][k][i + 2] *= alpha;
+            }
+          }
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float top = m[n][i & 1];
+          s[n][i] = ex2(s[n][i] - (top == -INFINITY ? 0.f : top));
+        }
+        l[n][0] += s[n][0] + s[n][2];
+        l[n][1] += s[n][1] + s[n][3];
+        pf[n][0] = pack2<T>(s[n][0], s[n][1]);
+        pf[n][1] = pack2<T>(s[n][2], s[n][3]);
+      }
+      if (some_masked && p.Sq > 1) {
+        // A weight of zero does not silence a NaN or an infinity in V in the product below. Keys that only
+        // the later tokens see are taken out of it when their V is not finite, and added by hand
+        // to the rows that do see them.
+        bool odd = false;
+        for (int r = max(0, at.len - p.Sq + 1 - key0); r < SUB && (mask >> r & 1); ++r)
+          for (int c = lane; c < DP; c += 32) {
+            const float v = bits_to_f32<T>(reinterpret_cast<const unsigned short*>(ring_ptr + stage * STAGE_BYTES + V_OFF + r * (DP * 2))[c]);
+            odd |= !(fabsf(v) < INFINITY);
+          }
+        if (__any_sync(0xffffffffu, odd)) {
+          for (int r = max(0, at.len - p.Sq + 1 - key0); r < SUB; ++r) {
+            char* const row = ring_ptr + stage * STAGE_BYTES + V_OFF + r * (DP * 2);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint32_t two = __shfl_sync(0xffffffffu, r < 8 ? pf[n][0] : pf[n][1], (r & 7) * 4 + t4);
+              const float p0 = bits_to_f32<T>(two & 0xffffu), p1 = bits_to_f32<T>(two >> 16);
+#pragma unroll
+              for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const float v = bits_to_f32<T>(*reinterpret_cast<const unsigned short*>(row + (((k * 2 + i) ^ (r & 7)) << 4) + g * 2));
+                  if (p0 != 0.f) acc[n][k][i * 2] = fmaf(p0, v, acc[n][k][i * 2]);
+                  if (p1 != 0.f) acc[n][k][i * 2 + 1] = fmaf(p1, v, acc[n][k][i * 2 + 1]);
+                }
+            }
+            __syncwarp();
+            for (int c = lane; c < DP / 2; c += 32) reinterpret_cast<uint32_t*>(row)[c] = 0u;
+          }
+          __syncwarp();
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        pf[n][0] = movmatrix_trans(pf[n][0]);
+        pf[n][1] = movmatrix_trans(pf[n][1]);
+      }
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) {
+        uint32_t a[4];
+        ldmatrix4_trans(a, base + V_OFF + vrow * (DP * 2) + (((k * 2 + vchunk) ^ (vrow & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<T>(acc[n][k], a, pf[n][0], pf[n][1]);
+      }
+    }
+    __syncwarp();
+    fetch(stage);
+    cp_async_commit();
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+    if (++at.t < at.tiles && left > 1) continue;
+    // ---- the CTA leaves the unit: join the four warps, in turn so that the order is fixed
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+        if (g == 0) {
+          wm[warp][n * 8 + t4 * 2 + i] = m[n][i];
+          wl[warp][n * 8 + t4 * 2 + i] = l[n][i];
+        }
+      }
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+      if (w == warp) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = n * 8 + t4 * 2 + i;
+            const float top = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+            const float scale = exp2_safe(m[n][i], top);
+#pragma unroll
+            for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float* o = obuf + r * OB + k * 16 + e * 8 + g;
+                *o = w == 0 ? acc[n][k][e * 2 + i] * scale : fmaf(acc[n][k][e * 2 + i], scale, *o);
+              }
+          }
+      }
+      __syncthreads();
+    }
+    const int64_t slot = partial_slot(t0, at.t, at.tiles);
+    for (int r = warp; r < nrows; r += 4) {
+      const int row = row0 + r;
+      const float top = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum = fmaf(wl[w][r], exp2_safe(wm[w][r], top), sum);
+      if (slot < 0) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key has no weight: zeros
+        const int64_t out = at.b * p.sob + row_head(p, hkv, row) * p.soh + row_token(p, row) * p.sos;
+        for (int d = lane; d < p.D; d += 32) store_from_f32(p.o, p.o_dtype, out + d, obuf[r * OB + d] * inv);
+      } else {
+        if (lane == 0) p.ml[slot * p.unit_rows + r] = make_float2(top, sum);
+        for (int d = lane; d < p.D; d += 32) p.part[(slot * p.unit_rows + r) * p.Dp + d] = obuf[r * OB + d];
+      }
+    }
+    __syncthreads();
+    fresh = true;
+    if (left > 1) at.next_unit(p);
+  }
+}
+
+template <int DP>
+constexpr int n_tiles_max() { return DP == 256 ? 2 : 4; }
+
+// Query rows of a unit: eight, sixteen or thirty-two, whichever takes the rows of a kv head in
+// the fewest passes over its keys (32 x 256 accumulators would not fit the registers).
+int n_tiles_for(int rows, int D) {
+  const int most = D > 128 ? 2 : 4;
+  return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
+}
+
+typedef void (*PagedKernel)(const PagedParams);
+template <typename T, int DP, int NT>
+int launch(lh_ctx* ctx, const PagedParams& p, int ctas) {
+  constexpr int smem = 4 * Shape<DP>::stages * Shape<DP>::stage_bytes + NT * 8 * (DP + 4) * 4;
+  PagedKernel kernel = p.page % SUB == 0 ? paged_mma_kernel<T, DP, NT, true> : paged_mma_kernel<T, DP, NT, false>;
+  LH_CUDA_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<static_cast<unsigned>(ctas), THREADS, smem, ctx->stream>>>(p);
+  LH_CHECK_LAUNCH(ctx, "paged_mma_kernel");
+  return LH_OK;
+}
+template <typename T>
+int launch_type(lh_ctx* ctx, const PagedParams& p, int ctas) {
+  const int nt = p.unit_rows / 8;
+  if (p.D <= 64) return nt == 1 ? launch<T, 64, 1>(ctx, p, ctas) : nt == 2 ? launch<T, 64, 2>(ctx, p, ctas) : launch<T, 64, 4>(ctx, p, ctas);
+  if (p.D <= 128) return nt == 1 ? launch<T, 128, 1>(ctx, p, ctas) : nt == 2 ? launch<T, 128, 2>(ctx, p, ctas) : launch<T, 128, 4>(ctx, p, ctas);
+  return nt == 1 ? launch<T, 256, 1>(ctx, p, ctas) : launch<T, 256, 2>(ctx, p, ctas);
+}
+
+}  // namespace
+
+int paged_mma_unit_rows(int64_t rows, int D) { return 8 * n_tiles_for(rows > 64 ? 64 : static_cast<int>(rows), D); }
+int paged_mma_ctas(const lh_ctx* ctx, int D) { return ctx->sm_count * (D > 128 ? Shape<256>::ctas_per_sm : Shape<128>::ctas_per_sm); }
+
+bool paged_mma_supported(const lh_memref_t* k, const lh_memref_t* v) {
+  if ((k->dtype != LH_BF16 && k->dtype != LH_F16) || k->shape[3] % 8) return false;
+  for (const lh_memref_t* m : {k, v}) {
+    if (reinterpret_cast<uintptr_t>(data_ptr(m)) % 16) return false;
+    for (int i = 0; i < 3; ++i)
+      if (m->shape[i] > 1 && m->strides[i] % 8) return false;
+  }
+  return true;
+}
+
+int paged_mma_launch(lh_ctx* ctx, PagedParams& p, int dtype, int ctas) {
+  p.tile = TILE;
+  return dtype == LH_BF16 ? launch_type<__nv_bfloat16>(ctx, p, ctas) : launch_type<__half>(ctx, p, ctas);
+}
+
+}  // namespace lh
