@@ -5,8 +5,20 @@
 // drawn token does not depend on how the row was cut up. In f32 the running sum of 10^5 weights
 // is off by 1e-7 of the total, and as many borders between tokens lie in it: one row in some
 // hundreds would get another token than the definition gives.
+//
+// A row belongs to a cluster of CTAs and stays in their shared memory: it is read once. What top-k
+// and top-p keep is always "the first so many in the order of falling logits, equal ones by
+// rising index", so each is one border in that order. It is found by a histogram of the
+// row over log2 of the weight (4096 bins of 1/93 octave): the bin that the border falls in
+// holds a few dozen tokens, which are collected in one CTA and ranked against each other.
+// Bins too full for that (rows of equal logits) are first split by further digits of the
+// order itself. The CTAs talk through distributed shared memory.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "epilogue.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace lh {
 namespace {
@@ -14,6 +26,7 @@ namespace {
 struct SampleParams {
   const void* logits; int64_t row_stride; int dtype;
   int rows, vocab;
+  int items;  // values per thread: a CTA has items * SAMPLE_THREADS of the row
   const float* uniform; int64_t su;
   const float* temperature; int64_t st;
   const void* top_k; int64_t sk; int k64;
@@ -23,11 +36,18 @@ struct SampleParams {
   float* logprobs; int64_t slp;
 };
 
-constexpr double WEIGHT_ONE = 4398046511104.0;  // 2^42: the largest weight
+typedef unsigned long long u64;
+
 constexpr int WEIGHT_BITS = 42;
-constexpr int64_t MAX_VOCAB = int64_t(1) << 20;  // 2^20 weights of 2^42 stay within 63 bits
-constexpr int SAMPLE_THREADS = 1024;
+constexpr u64 WEIGHT_ONE = 1ull << WEIGHT_BITS;  // the largest weight
+constexpr int INDEX_BITS = 20;
+constexpr int64_t MAX_VOCAB = int64_t(1) << INDEX_BITS;  // 2^20 weights of 2^42 stay within 63 bits
+constexpr int SAMPLE_THREADS = 512;
 constexpr int WARPS = SAMPLE_THREADS / 32;
+constexpr int MAX_CLUSTER = 8;
+constexpr int BINS = 4096;
+constexpr float BINS_PER_OCTAVE = 93.f;  // the last bin starts 44 octaves below the maximum: weights of zero
+constexpr int LIST = SAMPLE_THREADS;
 
 // Values in an order that whole numbers keep; NaN ranks with -inf, -0 with +0.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -36,18 +56,37 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu)); }
+// Position in the order of falling logits and rising index: larger comes first, no two are equal.
+__device__ __forceinline__ u64 order_of(float x, int i) { return (static_cast<u64>(key_of(x)) << INDEX_BITS) | (MAX_VOCAB - 1 - i); }
+__device__ __forceinline__ int index_of(u64 order) { return static_cast<int>(MAX_VOCAB - 1 - (order & (MAX_VOCAB - 1))); }
+__device__ __forceinline__ float logit_of(u64 order) { return value_of(static_cast<uint32_t>(order >> INDEX_BITS)); }
+
+constexpr int TABLE = 256;
 
 struct Weighing {
-  double top, scale;  // row maximum, log2(e) / T
-  // log2 of the weight: 0 for the maximum
-  __device__ __forceinline__ double log2_of(float x) const {
-    const double d = static_cast<double>(x);
-    return d == top ? 0.0 : (d - top) * scale;
+  float top;
+  double top64, scale;   // row maximum; 256 log2(e) / T
+  float bin_scale;       // bins per two units of logit
+  const double* table;   // 2^(42 + i / 256)
+  // 2^t = 2^(j / 256) (1 + (e^(f ln2 / 256) - 1)), 256 t = j + f, |f| <= 1/2: the series' fourth term
+  // and on are below 2^-42. Adding 2^52 leaves the rounded whole number in the low bits.
+  __device__ __forceinline__ u64 of(float x) const {
+    const double y = x == top ? 0.0 : (static_cast<double>(x) - top64) * scale;
+    if (!(y > -(WEIGHT_BITS + 1.0) * TABLE)) return 0;  // also NaN, and (-inf) * 0
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52
+    const double z = y + magic;
+    const int j = __double2loint(z);
+    const double f = y - (z - magic);
+    const double a1 = 0.69314718055994530942 / TABLE;
+    const double s = f * fma(f, fma(f, a1 * a1 * a1 / 6, a1 * a1 / 2), a1);
+    const double base = table[j & (TABLE - 1)];
+    const double scaled = __hiloint2double(__double2hiint(base) + (j >> 8) * (1 << 20), __double2loint(base));
+    const double fixed = fma(scaled, s, scaled) + 4503599627370496.0;
+    return static_cast<u64>(__double_as_longlong(fixed)) & ((1ull << 52) - 1);
   }
-  __device__ __forceinline__ unsigned long long of(float x) const {
-    const double t = log2_of(x);
-    if (!(t > -(WEIGHT_BITS + 1.0)) || x == -INFINITY) return 0;  // also NaN: (-inf) * 0
-    return static_cast<unsigned long long>(__double2ll_rn(exp2(t) * WEIGHT_ONE));
+  // Falls with x. The last bin is for weights of zero. (Halves: the difference stays finite.)
+  __device__ __forceinline__ int bin_of(float x) const {
+    return x == top ? 0 : static_cast<int>(fminf((0.5f * top - 0.5f * x) * bin_scale, static_cast<float>(BINS - 1)));  // NaN: the last
   }
 };
 
@@ -58,221 +97,301 @@ __device__ __forceinline__ V warp_total(V v) {
   return v;
 }
 
-__device__ unsigned long long block_total(unsigned long long v, unsigned long long* red) {
+struct SampleShared {
+  double table[TABLE];
+  u64 hist[BINS];
+  u64 list[LIST], mass[LIST];
+  u64 from[4][MAX_CLUSTER];  // what each CTA of the cluster sent, per use
+  u64 red[WARPS];
+  u64 border, above;         // answers of the first CTA
+  int bin, listed;
+  int found;
+};
+
+// One CTA's part of a row. HELD: its values lie in shared memory; otherwise each pass reads them
+// from global memory again (from L2: a cluster's row is in use by nobody else).
+template <bool HELD>
+struct Row {
+  const float* held;
+  const void* logits; int dtype; int64_t base;
+  int offset, first, steps, vocab;  // this lane's place in the CTA's part and in the row, how many values it has (32 apart)
+  __device__ __forceinline__ float value(int j) const {
+    return HELD ? held[offset + j * 32] : load_as_f32(logits, dtype, base + first + j * 32);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll 4
+    for (int j = 0; j < steps; ++j) {
+      const int i = first + j * 32;
+      if (i < vocab) f(value(j), i);
+    }
+  }
+};
+
+__device__ __forceinline__ u64 block_total(u64 v, u64* red) {
   v = warp_total(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0;
+#pragma unroll
   for (int w = 0; w < WARPS; ++w) v += red[w];
   return v;
 }
 
-// One CTA per row; each warp owns a run of the row, so that index order is warp order.
-__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleParams p) {
-  __shared__ unsigned long long red[WARPS];
-  __shared__ unsigned long long mass[256];
-  __shared__ int count[256];
-  __shared__ unsigned long long sh_mass;
-  __shared__ int sh_digit, sh_count, sh_index;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x;
-  const int64_t base = row * p.row_stride;
-  const int run = ((p.vocab + WARPS - 1) / WARPS + 31) / 32 * 32;
-  const int w0 = min(warp * run, p.vocab), w1 = min(w0 + run, p.vocab);
-  auto value = [&](int i) { return load_as_f32(p.logits, p.dtype, base + i); };
-  auto finish = [&](int64_t token, float lp) {
-    if (tid == 0) {
-      if (p.tok64) static_cast<int64_t*>(p.tokens)[row * p.stok] = token;
-      else static_cast<int32_t*>(p.tokens)[row * p.stok] = static_cast<int32_t>(token);
-      if (p.logprobs) p.logprobs[row * p.slp] = lp;
-    }
-  };
-  // the largest key, and the first index that has it
-  unsigned long long best = 0;
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const unsigned long long k = (static_cast<unsigned long long>(key_of(value(i))) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
-    if (k > best) best = k;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, d);
-    if (o > best) best = o;
-  }
-  if (lane == 0) red[warp] = best;
-  __syncthreads();
-  best = 0;
-  for (int w = 0; w < WARPS; ++w) best = red[w] > best ? red[w] : best;
-  const uint32_t key_max = static_cast<uint32_t>(best >> 32);
-  const int first_max = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
-  const float top = value_of(key_max);
-  if (top == -INFINITY) return finish(-1, -INFINITY);
-  const float temperature = p.temperature ? p.temperature[row * p.st] : 1.f;
-  const float top_p = p.top_p ? p.top_p[row * p.sp] : 1.f;
-  const float min_p = p.min_p ? p.min_p[row * p.sm] : 0.f;
-  int64_t k = p.top_k ? (p.k64 ? static_cast<const int64_t*>(p.top_k)[row * p.sk] : static_cast<const int32_t*>(p.top_k)[row * p.sk]) : 0;
-  if (!(temperature > 0.f) || k == 1 || top_p <= 0.f) return finish(first_max, 0.f);
-  Weighing weigh;
-  weigh.top = static_cast<double>(top);
-  weigh.scale = 1.4426950408889634073599 / static_cast<double>(temperature);
+// Every CTA's value reaches every CTA; `use` numbers the exchanges of a row.
+__device__ __forceinline__ void exchange(const cg::cluster_group& cluster, SampleShared& sh, int use, u64 v) {
+  const unsigned n = cluster.num_blocks();
+  if (threadIdx.x < n) cluster.map_shared_rank(&sh.from[use][cluster.block_rank()], threadIdx.x)[0] = v;
+  cluster.sync();
+}
 
-  // Kept so far: keys above `key`, and the first `ties` of those equal to it.
-  uint32_t key = 0;
-  int64_t ties = p.vocab;
-  if (k > 0 && k < p.vocab) {
-    // the k-th largest key, eight bits at a time
-    int64_t left = k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) count[tid] = 0;
-      __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t q = key_of(value(i));
-        if ((q & mask) == key) atomicAdd(&count[(q >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int d = 255;
-        int64_t rest = left;
-        while (d > 0 && count[d] < rest) rest -= count[d--];
-        sh_digit = d;
-        sh_count = static_cast<int>(rest);
-      }
-      __syncthreads();
-      key |= static_cast<uint32_t>(sh_digit) << shift;
-      left = sh_count;
-      __syncthreads();
-    }
-    ties = left;
-  }
-  if (top_p < 1.f) {
-    // total weight of what is left, then the key at which the running sum, taken from the largest
-    // weight down, reaches its share
-    unsigned long long sum = 0;
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const float x = value(i);
-      if (key_of(x) > key) sum += weigh.of(x);
-    }
-    sum = block_total(sum, red);
-    if (key) sum += static_cast<unsigned long long>(ties) * weigh.of(value_of(key));
-    // a whole number reaches p * sum when it reaches the next whole number
-    const unsigned long long need = __double2ull_ru(static_cast<double>(top_p) * static_cast<double>(sum));
-    unsigned long long above = 0;
-    uint32_t at = 0;
-    int64_t equal = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) { mass[tid] = 0; count[tid] = 0; }
-      __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = w0 + lane; i < w1; i += 32) {
-        const float x = value(i);
-        const uint32_t q = key_of(x);
-        if ((q & mask) == at && q >= key) {
-          atomicAdd(&mass[(q >> shift) & 255], weigh.of(x));
-          atomicAdd(&count[(q >> shift) & 255], 1);
-        }
-      }
-      __syncthreads();
-      if (tid == 0) {
-        // p < 1 keeps `need` within the sum, and ties of `key` beyond the first `ties`, which are
-        // not in the sum, lie in the last bin that holds anything: the walk ends in a bin
-        unsigned long long run_sum = above;
-        int d = 255;
-        while (d > 0 && run_sum + mass[d] < need) run_sum += mass[d--];
-        sh_digit = d;
-        sh_mass = run_sum;
-        sh_count = count[d];
-      }
-      __syncthreads();
-      at |= static_cast<uint32_t>(sh_digit) << shift;
-      above = sh_mass;
-      equal = sh_count;
-      __syncthreads();
-    }
-    if (at > key || !key) ties = equal;  // all of them, before the share is counted
-    key = at;
-    const unsigned long long each = weigh.of(value_of(key));
-    // each > 0: `above` alone falls short of `need`
-    const int64_t want = static_cast<int64_t>((need - above + each - 1) / each);
-    if (want < ties) ties = want;
-  }
-  // the index of the last tie that is kept
-  int last_tie = p.vocab;
-  if (key) {
-    int here = 0;
-    for (int i = w0 + lane; i < w1; i += 32) here += key_of(value(i)) == key;
-    here = warp_total(here);
+// The border of a filter: the `want`-th token in order (BY_MASS false), or the first at which the
+// running weight reaches `want`. Only tokens at or above `floor` and in bins up to `last_bin`
+// count. 0: the border lies among weights of zero.
+template <bool BY_MASS, typename R>
+__device__ u64 find_border(const cg::cluster_group& cluster, SampleShared& sh, const R& row, const Weighing& weigh, u64 want, u64 floor, int last_bin) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  SampleShared& lead = *cluster.map_shared_rank(&sh, 0);
+  const bool is_lead = cluster.block_rank() == 0;
+  uint32_t* const count = reinterpret_cast<uint32_t*>(sh.hist);
+  u64 prefix = 0, prefix_mask = 0;
+  int only_bin = -1;
+  for (int shift = 64;;) {  // first the bins, then 12 bits of the order at a time from the top
+    for (int i = tid; i < BINS; i += SAMPLE_THREADS) sh.hist[i] = 0;
+    if (is_lead && tid == 0) sh.listed = 0;
+    cluster.sync();  // the first CTA's histogram is empty before any other adds to it
+    row.each([&](float x, int i) {
+      const int b = weigh.bin_of(x);
+      if (b > last_bin || (only_bin >= 0 && b != only_bin)) return;
+      const u64 o = order_of(x, i);
+      if (o < floor || (o & prefix_mask) != prefix) return;
+      const int at = shift == 64 ? b : BINS - 1 - static_cast<int>((o >> shift) & (BINS - 1));
+      if (BY_MASS) atomicAdd(&sh.hist[at], weigh.of(x));
+      else atomicAdd(&count[at], 1u);
+    });
     __syncthreads();
-    if (lane == 0) red[warp] = static_cast<unsigned long long>(here);
-    if (tid == 0) sh_index = p.vocab;
-    __syncthreads();
-    int64_t before = 0;
-    for (int w = 0; w < warp; ++w) before += static_cast<int64_t>(red[w]);
-    if (before < ties && before + here >= ties) {
-      int64_t seen = before;
-      for (int i0 = w0; i0 < w1; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned hit = __ballot_sync(0xffffffffu, i < w1 && key_of(value(i)) == key);
-        if (seen + __popc(hit) >= ties) {
-          const int nth = static_cast<int>(ties - seen);  // the nth set bit
-          if ((hit >> lane & 1) && __popc(hit & ((2u << lane) - 1)) == nth) sh_index = i;
-          break;
-        }
-        seen += __popc(hit);
+    if (!is_lead) {
+      uint32_t* const lead_count = reinterpret_cast<uint32_t*>(lead.hist);
+      for (int i = tid; i < BINS; i += SAMPLE_THREADS) {
+        if (BY_MASS) { if (sh.hist[i]) atomicAdd(&lead.hist[i], sh.hist[i]); }
+        else { if (count[i]) atomicAdd(&lead_count[i], count[i]); }
       }
     }
-    __syncthreads();
-    last_tie = sh_index;
-  }
-  const double floor2 = min_p > 0.f ? log2(static_cast<double>(min_p)) : -INFINITY;
-  auto kept_weight = [&](int i) -> unsigned long long {
-    const float x = value(i);
-    const uint32_t q = key_of(x);
-    if (q < key || (q == key && i > last_tie)) return 0;
-    if (!(x == x)) return 0;
-    if (q != key_max && !(weigh.log2_of(x) >= floor2)) return 0;
-    return weigh.of(x);
-  };
-  unsigned long long mine = 0;
-  for (int i = w0 + lane; i < w1; i += 32) mine += kept_weight(i);
-  mine = warp_total(mine);
-  __syncthreads();
-  if (lane == 0) red[warp] = mine;
-  if (tid == 0) sh_index = -1;
-  __syncthreads();
-  unsigned long long total = 0, before = 0;
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += red[w];
-    total += red[w];
-  }
-  // the first index whose running sum is above u * total; a number at or beyond 1 takes the last
-  const float u = p.uniform[row * p.su];
-  const unsigned long long target = !(u > 0.f) ? 0 : u >= 1.f ? total - 1 : __double2ull_rd(static_cast<double>(u) * static_cast<double>(total));
-  if (before <= target && before + mine > target) {
-    unsigned long long sum = before;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const int i = i0 + lane;
-      const unsigned long long w = i < w1 ? kept_weight(i) : 0;
-      unsigned long long incl = w;
+    cluster.sync();
+    if (is_lead) {
+      constexpr int RUN = BINS / SAMPLE_THREADS;
+      u64 mine = 0;
+#pragma unroll
+      for (int i = 0; i < RUN; ++i) mine += BY_MASS ? sh.hist[tid * RUN + i] : count[tid * RUN + i];
+      u64 incl = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, d);
+        const u64 up = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += up;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, sum + incl > target);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          sh_index = i;
-          sh_mass = w;
+      if (lane == 31) sh.red[warp] = incl;
+      if (tid == 0) sh.found = -1;
+      __syncthreads();
+      u64 sum = incl - mine;
+      for (int w = 0; w < warp; ++w) sum += sh.red[w];
+      if (sum < want && want <= sum + mine) {
+        int b = tid * RUN;
+        for (;; ++b) {
+          const u64 here = BY_MASS ? sh.hist[b] : count[b];
+          if (want <= sum + here) break;
+          sum += here;
         }
-        break;
+        sh.found = b;
+        sh.above = sum;
       }
-      sum += __shfl_sync(0xffffffffu, incl, 31);
+      __syncthreads();
+      if (tid < static_cast<int>(cluster.num_blocks())) {
+        SampleShared& other = *cluster.map_shared_rank(&sh, tid);
+        other.bin = sh.found;
+        if (tid) other.above = sh.above;
+      }
+    }
+    cluster.sync();
+    const int bin = sh.bin;
+    if (bin < 0) return 0;
+    want -= sh.above;
+    if (shift == 64) only_bin = bin;
+    else {
+      prefix |= static_cast<u64>(BINS - 1 - bin) << shift;
+      prefix_mask |= static_cast<u64>(BINS - 1) << shift;
+    }
+    // the bin's tokens, ranked by the first CTA if they are few enough
+    row.each([&](float x, int i) {
+      if (weigh.bin_of(x) != only_bin) return;
+      const u64 o = order_of(x, i);
+      if (o < floor || (o & prefix_mask) != prefix) return;
+      const int at = atomicAdd(&lead.listed, 1);
+      if (at < LIST) {
+        lead.list[at] = o;
+        if (BY_MASS) lead.mass[at] = weigh.of(x);
+      }
+    });
+    cluster.sync();
+    const int listed = lead.listed;
+    if (listed <= LIST) {
+      if (is_lead) {
+        if (tid < listed) {
+          const u64 o = sh.list[tid];
+          u64 before = 0;
+          for (int i = 0; i < listed; ++i)
+            if (sh.list[i] > o) before += BY_MASS ? sh.mass[i] : 1;
+          if (before < want && want <= before + (BY_MASS ? sh.mass[tid] : 1)) sh.border = o;
+        }
+        __syncthreads();
+        if (tid > 0 && tid < static_cast<int>(cluster.num_blocks())) cluster.map_shared_rank(&sh, tid)->border = sh.border;
+      }
+      cluster.sync();
+      return sh.border;
+    }
+    shift = shift == 64 ? 40 : shift > 12 ? shift - 12 : 0;  // 52 bits: 40, 28, 16, 4, 0
+    cluster.sync();  // everyone has read `listed` before it is cleared
+  }
+}
+
+template <bool HELD>
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleParams p) {
+  __shared__ SampleShared sh;
+  extern __shared__ float held[];
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();  // waited for below: nobody writes to a CTA that has not started
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int r = blockIdx.x / ctas;
+  Row<HELD> row;
+  row.held = held;
+  row.logits = p.logits;
+  row.dtype = p.dtype;
+  row.base = r * p.row_stride;
+  row.vocab = p.vocab;
+  row.steps = p.items;
+  row.offset = warp * 32 * p.items + lane;  // a warp owns a run: index order is CTA, warp, step, lane
+  row.first = rank * SAMPLE_THREADS * p.items + row.offset;
+  if (HELD) {
+#pragma unroll 16
+    for (int j = 0; j < p.items; ++j) {
+      const int i = row.first + j * 32;
+      held[row.offset + j * 32] = i < p.vocab ? load_as_f32(p.logits, p.dtype, row.base + i) : 0.f;  // only this lane reads it back
     }
   }
+  if (tid < TABLE) sh.table[tid] = exp2(WEIGHT_BITS + static_cast<double>(tid) / TABLE);
+  auto finish = [&](int64_t token, float lp) {
+    if (p.tok64) static_cast<int64_t*>(p.tokens)[r * p.stok] = token;
+    else static_cast<int32_t*>(p.tokens)[r * p.stok] = static_cast<int32_t>(token);
+    if (p.logprobs) p.logprobs[r * p.slp] = lp;
+  };
+  // the first in order
+  u64 best = 0;
+  row.each([&](float x, int i) {
+    const u64 o = order_of(x, i);
+    if (o > best) best = o;
+  });
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    const u64 o = __shfl_xor_sync(0xffffffffu, best, d);
+    if (o > best) best = o;
+  }
+  if (lane == 0) sh.red[warp] = best;
   __syncthreads();
-  finish(sh_index, static_cast<float>(log(static_cast<double>(sh_mass) / static_cast<double>(total))));
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) best = sh.red[w] > best ? sh.red[w] : best;
+  cluster.barrier_wait();
+  exchange(cluster, sh, 0, best);
+  for (int c = 0; c < ctas; ++c) best = sh.from[0][c] > best ? sh.from[0][c] : best;
+  const float top = logit_of(best);
+  const float temperature = p.temperature ? p.temperature[r * p.st] : 1.f;
+  const float top_p = p.top_p ? p.top_p[r * p.sp] : 1.f;
+  const float min_p = p.min_p ? p.min_p[r * p.sm] : 0.f;
+  const int64_t k = p.top_k ? (p.k64 ? static_cast<const int64_t*>(p.top_k)[r * p.sk] : static_cast<const int32_t*>(p.top_k)[r * p.sk]) : 0;
+  if (top == -INFINITY || !(temperature > 0.f) || k == 1 || top_p <= 0.f) {  // the whole cluster leaves; nobody's memory is asked for any more
+    if (rank == 0 && tid == 0) {
+      if (top == -INFINITY) finish(-1, -INFINITY);
+      else finish(index_of(best), 0.f);
+    }
+    return;
+  }
+  Weighing weigh;
+  weigh.top = top;
+  weigh.top64 = static_cast<double>(top);
+  weigh.scale = TABLE * 1.4426950408889634073599 / static_cast<double>(temperature);
+  weigh.bin_scale = 2.f * BINS_PER_OCTAVE * 1.44269504f / temperature;
+  weigh.table = sh.table;
+
+  u64 border = 0;  // kept: this place in the order and before
+  if (k > 0 && k < p.vocab) border = find_border<false>(cluster, sh, row, weigh, static_cast<u64>(k), 0, BINS - 2);
+  if (top_p < 1.f) {
+    u64 sum = 0;
+    row.each([&](float x, int i) {
+      if (order_of(x, i) >= border) sum += weigh.of(x);
+    });
+    sum = block_total(sum, sh.red);
+    exchange(cluster, sh, 1, sum);
+    sum = 0;
+    for (int c = 0; c < ctas; ++c) sum += sh.from[1][c];
+    // a whole number reaches p * sum when it reaches the next whole number; p < 1 keeps that within the sum
+    const u64 need = __double2ull_ru(static_cast<double>(top_p) * static_cast<double>(sum));
+    // Tokens lighter than (sum - need) / vocab are beyond the border: all together they do not make
+    // up what may be left out. One bin of margin covers the bins' f32 arithmetic.
+    const u64 light = (sum - need) / static_cast<u64>(p.vocab);
+    int last_bin = BINS - 2;
+    if (light > 0) last_bin = min(last_bin, static_cast<int>((WEIGHT_BITS - log2f(static_cast<float>(light))) * BINS_PER_OCTAVE) + 2);
+    border = find_border<true>(cluster, sh, row, weigh, need, border, last_bin);
+  }
+  const u64 least = min_p > 0.f ? __double2ull_ru(fmin(static_cast<double>(min_p), 1.0) * static_cast<double>(WEIGHT_ONE)) : 0;
+  auto kept_weight = [&](float x, int i) -> u64 {
+    if (order_of(x, i) < border) return 0;
+    const u64 w = weigh.of(x);
+    return w >= least ? w : 0;  // the largest weighs 2^42: it always stays
+  };
+  u64 mine = 0;
+  row.each([&](float x, int i) { mine += kept_weight(x, i); });
+  mine = warp_total(mine);
+  __syncthreads();
+  if (lane == 0) sh.red[warp] = mine;
+  __syncthreads();
+  u64 here = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += sh.red[w];
+    here += sh.red[w];
+  }
+  exchange(cluster, sh, 2, here);
+  u64 total = 0;
+  for (int c = 0; c < ctas; ++c) {
+    if (c < rank) before += sh.from[2][c];
+    total += sh.from[2][c];
+  }
+  // the first index whose running sum is above u * total; a number at or beyond 1 takes the last
+  const float u = p.uniform[r * p.su];
+  const u64 target = !(u > 0.f) ? 0 : u >= 1.f ? total - 1 : __double2ull_rd(static_cast<double>(u) * static_cast<double>(total));
+  if (before <= target && before + mine > target) {  // one warp of the cluster
+    for (int j = 0; j < p.items; ++j) {
+      const int i = row.first + j * 32;
+      const u64 w = i < p.vocab ? kept_weight(load_as_f32(p.logits, p.dtype, row.base + i), i) : 0;
+      u64 incl = w;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const u64 up = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += up;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > target);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) finish(i, static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total))));
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
 }
+
+// Values per thread that fit a CTA's shared memory beside its tables; with 32 or fewer two CTAs
+// share an SM, and one loads while the other computes.
+constexpr int MOST_HELD = 64;
 
 bool vector_of(const lh_memref_t* m, int64_t n) { return m->rank == 1 && m->shape[0] == n; }
 
@@ -316,8 +435,31 @@ extern "C" int lh_b200_sample(lh_ctx_t* ctx, const lh_memref_t* tokens, const lh
   p.logprobs = f32(logprobs, p.slp);
   if (top_k) { p.top_k = data_ptr(top_k); p.sk = top_k->strides[0]; p.k64 = top_k->dtype == LH_I64; }
   p.tokens = data_ptr(tokens); p.stok = tokens->strides[0]; p.tok64 = tokens->dtype == LH_I64;
+  // Small rows take one CTA. Larger ones take up to eight, four values per thread and more: what a
+  // row costs is mostly latency (barriers, histograms), so the wider it is spread the sooner it
+  // ends, and eight is the largest cluster that every launch may have.
+  int ctas = 1;
+  while (ctas < MAX_CLUSTER && v > static_cast<int64_t>(ctas) * SAMPLE_THREADS * 4) ctas *= 2;
+  p.items = static_cast<int>((v + static_cast<int64_t>(ctas) * SAMPLE_THREADS - 1) / (static_cast<int64_t>(ctas) * SAMPLE_THREADS));
+  if (n > 0x7fffffffll / ctas) return set_error(ctx, LH_ERR_UNSUPPORTED, "sample: %lld rows are too many for one call", (long long)n);
   DeviceScope scope(ctx->device);
-  sample_kernel<<<static_cast<unsigned>(n), SAMPLE_THREADS, 0, ctx->stream>>>(p);
+  const bool held = p.items <= MOST_HELD;
+  const size_t smem = held ? static_cast<size_t>(p.items) * SAMPLE_THREADS * sizeof(float) : 0;
+  if (held) LH_CUDA_CHECK(ctx, cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_HELD * SAMPLE_THREADS * static_cast<int>(sizeof(float))));
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(n * ctas));
+  cfg.blockDim = dim3(SAMPLE_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LH_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, held ? sample_kernel<true> : sample_kernel<false>, p));
   LH_CHECK_LAUNCH(ctx, "sample_kernel");
   return LH_OK;
 }

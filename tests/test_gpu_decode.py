@@ -438,3 +438,15 @@ def test_sample_refusals(ctx):
                                           (t, torch.zeros(1, 1, device="cuda").expand(3, (1 << 20) + 1), u, {}), (t.cpu(), x, u, {})):
         with pytest.raises(ValueError):
             ctx.sample(tokens, logits, uniform, **more)
+
+
+@pytest.mark.parametrize("vocab", [200000, 400000, (1 << 20) - 3, 1 << 20])
+def test_sample_wide_rows(ctx, vocab):
+    """Rows that do not fit the cluster's shared memory at two CTAs an SM, and rows that do not fit it at all."""
+    rng = np.random.default_rng(vocab)
+    logits = randn(rng, 3, vocab) * 2.5
+    logits[1] = torch.round(logits[1])
+    u = rng.random(3, dtype=np.float32)
+    check_sample(ctx, logits, u, top_k=[70, 100000, vocab - 1], top_p=[0.9, 0.7, 0.99])
+    check_sample(ctx, logits, u, top_p=[0.9, 0.7, 0.99])
+    check_sample(ctx, logits, u)
