@@ -23,7 +23,6 @@
 // the histogram goes by an f32 coordinate. Running sums are kept in f64 with 2^52 added: adding
 // with rounding down then drops each weight's fraction, whatever the sum so far.
 #include <cooperative_groups.h>
-#include <stdlib.h>
 
 #include "common.cuh"
 
@@ -47,15 +46,13 @@ struct SampleParams {
 
 typedef unsigned long long u64;
 
-#ifndef OCC
-#define OCC 3
-#endif
 constexpr int WEIGHT_BITS = 42;
 constexpr u64 WEIGHT_ONE = 1ull << WEIGHT_BITS;  // the largest weight
 constexpr int INDEX_BITS = 20;
 constexpr int64_t MAX_VOCAB = int64_t(1) << INDEX_BITS;  // 2^20 weights of 2^42 stay within 63 bits
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
+constexpr int CTAS_PER_SM = 2;  // 64 registers: the weights' f64 chains interleave (three CTAs at 40 registers spill, and measured the same)
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_RUNS = MAX_CLUSTER * WARPS;
 constexpr int BINS = 4096;
@@ -606,7 +603,7 @@ struct Sampler {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, OCC) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) sample_kernel(const SampleParams p) {
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();  // waited for below: nobody writes to a CTA that has not started
@@ -851,11 +848,15 @@ extern "C" int lh_b200_sample(lh_ctx_t* ctx, const lh_memref_t* tokens, const lh
   p.logprobs = f32(logprobs, p.slp);
   if (top_k) { p.top_k = data_ptr(top_k); p.sk = top_k->strides[0]; p.k64 = top_k->dtype == LH_I64; }
   p.tokens = data_ptr(tokens); p.stok = tokens->strides[0]; p.tok64 = tokens->dtype == LH_I64;
+  // How many CTAs share a row. One row ends soonest on eight (131071 f32 values, top-p: 59 us on two
+  // CTAs, 40 on four, 30 on eight; eight is the largest cluster that every launch may have), but more CTAs
+  // than are resident at once wait for one another's clusters (64 such rows: 54 us on four, 68 on eight;
+  // 256: 178 on two, 199 on four). Rows of a few values per thread take fewer.
   const int64_t vec = 16 / static_cast<int64_t>(dtype_size(logits->dtype));
   const int64_t groups = v / vec > 0 ? v / vec : 1;  // whole ones; the odd ends are the first and the last warp's
-  int ctas = 1;
-  while (ctas < MAX_CLUSTER && groups > static_cast<int64_t>(ctas) * THREADS) ctas *= 2;
-  if (getenv("LH_C")) ctas = atoi(getenv("LH_C"));
+  const int64_t resident = static_cast<int64_t>(ctx->sm_count) * CTAS_PER_SM;
+  int ctas = groups > THREADS ? 2 : 1;
+  while (ctas > 1 && ctas < MAX_CLUSTER && groups > static_cast<int64_t>(ctas) * THREADS && n * ctas * 2 <= resident) ctas *= 2;
   p.steps = static_cast<int>((groups + static_cast<int64_t>(ctas) * THREADS - 1) / (static_cast<int64_t>(ctas) * THREADS));
   if (n > 0x7fffffffll / ctas) return set_error(ctx, LH_ERR_UNSUPPORTED, "sample: %lld rows are too many for one call", (long long)n);
   DeviceScope scope(ctx->device);
