@@ -111,6 +111,9 @@ int lh_b200_ctx_destroy(lh_ctx_t* ctx);
  * use_external == 0: return to the context's own stream (cuda_stream ignored). */
 int lh_b200_ctx_set_stream(lh_ctx_t* ctx, void* cuda_stream, int use_external);
 void* lh_b200_ctx_get_stream(lh_ctx_t* ctx);
+/* The stream that launches go to now (the side stream while that is selected), and whether it is
+ * being captured into a graph. Either result may be NULL. */
+int lh_b200_stream_info(lh_ctx_t* ctx, void** stream, int* capturing);
 /* Blocks until the stream is idle, then reads the device status word: returns
  * LH_ERR_DEVICE if a kernel gave up on a bounded wait since the last sync. */
 int lh_b200_sync(lh_ctx_t* ctx);

@@ -134,6 +134,7 @@ _PROTOTYPES = {
     "lh_b200_ctx_destroy": (c_int, [c_void_p]),
     "lh_b200_ctx_set_stream": (c_int, [c_void_p, c_void_p, c_int]),
     "lh_b200_ctx_get_stream": (c_void_p, [c_void_p]),
+    "lh_b200_stream_info": (c_int, [c_void_p, POINTER(c_void_p), POINTER(c_int)]),
     "lh_b200_sync": (c_int, [c_void_p]),
     "lh_b200_last_error": (c_char_p, [c_void_p]),
     "lh_b200_launch_count": (c_int64, [c_void_p]),
@@ -231,6 +232,35 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+_binding = None
+
+
+def binding():
+    """The CPython module ``lh_binding`` beside the library: ``call(fn, ctx, device, scalar, *operands)``
+    for operators whose kernels are shorter than filling their operands through ctypes."""
+    global _binding
+    if _binding is None:
+        import importlib.util
+
+        import torch
+
+        path = LIB_PATH.parent / "lh_binding.so"
+        if not path.exists():
+            raise RuntimeError(f"lighthouse_b200: {path} is missing; build it with `python -m lighthouse_b200.build`.")
+        spec = importlib.util.spec_from_file_location("lh_binding", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        codes = {torch.float32: LH_F32, torch.bfloat16: LH_BF16, torch.float16: LH_F16, torch.int32: LH_I32, torch.int64: LH_I64, torch.float64: LH_F64}
+        mod.setup(torch.Tensor, MemRef, codes)
+        _binding = mod
+    return _binding
+
+
+def address(name: str) -> int:
+    """Address of an exported entry point, for ``binding().call``."""
+    return ctypes.cast(getattr(load(), name), c_void_p).value
 
 
 class LighthouseCudaError(RuntimeError):

@@ -1,4 +1,5 @@
-"""Builds the in-tree native library ``lighthouse_b200/_lib/liblh_b200.so``.
+"""Builds the in-tree native library ``lighthouse_b200/_lib/liblh_b200.so`` and, beside it, the
+CPython module ``lh_binding.so`` (the short way into it for latency-bound operators).
 
 nvcc cross-compiles for sm_100a without a GPU, so this runs on any machine with
 the CUDA toolkit. Objects are rebuilt only when a source or header is newer.
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,6 +23,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 OBJ_DIR = LIB_DIR / "obj"
 LIB_PATH = LIB_DIR / "liblh_b200.so"
+BINDING_PATH = LIB_DIR / "lh_binding.so"
 INCLUDE = PKG_DIR.parent / "include"
 
 SOURCES = ["api.cu", "gemm_tc.cu", "gemm_simt.cu", "attention_tc2.cu", "attention_tc3.cu", "rowops.cu", "fused_collective.cu", "paged.cu", "paged_mma.cu", "sample.cu", "selftest.cu"]
@@ -62,9 +65,23 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose: bool) -> None:
         print(res.stderr, flush=True)
 
 
+def _build_binding(force: bool) -> None:
+    src = CSRC / "binding.c"
+    if not force and BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= max(src.stat().st_mtime, (INCLUDE / "lh_b200.h").stat().st_mtime):
+        return
+    include = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        raise RuntimeError(f"{include}/Python.h not found; the headers of this Python are required to build lighthouse_b200")
+    cmd = [shutil.which("gcc") or "cc", "-O2", "-shared", "-fPIC", "-I", include, "-o", str(BINDING_PATH), str(src)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     nvcc = find_nvcc()
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
+    _build_binding(force)
     header_mtime = _newest_header_mtime()
     jobs = []
     objs = []

@@ -68,6 +68,11 @@ class CudaContext:
         sm, major, minor = c_int(), c_int(), c_int()
         N.check(self._lib.lh_b200_device_info(self.handle, byref(sm), byref(major), byref(minor)), self.handle)
         self.sm_count, self.cc = sm.value, (major.value, minor.value)
+        self._entries: dict = {}
+        self._workspaces: dict = {}        # paged_attention's, by stream
+        self._workspaces_held: list = []
+        self._no_workspace = N.memref(0, (0,), (1,), N.LH_F32)
+        self._stream_info = (c_void_p(), c_int())
         if use_torch_stream:
             self.use_torch_stream()
 
@@ -189,18 +194,23 @@ class CudaContext:
         N.check(self._lib.lh_b200_embedding(self.handle, _ref(mo), _ref(mi), _ref(mw), _ref(mp), int(period)), self.handle, "lh_b200_embedding")
 
     # -- a decoding step's operators (see include/lh_b200.h for semantics) -------------------
-    def _on_device(self, *operands) -> None:
-        for t in operands:
-            if t is not None and not isinstance(t, N.MemRef) and t.is_cuda and t.device.index != self.device:
-                raise ValueError(f"an operand is on {t.device}, the context on cuda:{self.device}")
+    # These go through the compiled binding: their kernels take a few microseconds, and filling
+    # seven descriptors through ctypes would take 20.
+    def _entry(self, name: str):
+        """(call, address) of an entry point, looked up once."""
+        found = self._entries.get(name)
+        if found is None:
+            found = self._entries[name] = (N.binding().call, N.address(name))
+        return found
 
     def paged_append(self, q, k, v, k_pages, v_pages, slots, positions=None, theta: float = 10000.0) -> None:
         """New tokens' rows enter the paged cache: q (T, Hq, D), rotated in place, may be None;
         k, v (T, Hkv, D); pages (pages, page_size, Hkv, D); slots, positions (T) i32 or i64, a
         negative slot is padding. ``theta`` 0: no rotation."""
-        self._on_device(q, k, v, k_pages, v_pages, slots, positions)
-        m = [as_memref(t) for t in (q, k, v, k_pages, v_pages, slots, positions)]
-        N.check(self._lib.lh_b200_paged_append(self.handle, *map(_ref, m), float(theta)), self.handle, "lh_b200_paged_append")
+        call, fn = self._entry("lh_b200_paged_append")
+        rc = call(fn, self.handle.value, self.device, theta, q, k, v, k_pages, v_pages, slots, positions)
+        if rc:
+            N.check(rc, self.handle, "lh_b200_paged_append")
 
     def paged_attention_workspace(self, q, k_pages) -> int:
         """Bytes of workspace that ``paged_attention`` needs for operands of these shapes."""
@@ -214,40 +224,53 @@ class CudaContext:
         page_size, Hkv, D); page_table (B, columns), lengths (B) i32. ``workspace``: a CUDA
         tensor of ``paged_attention_workspace`` bytes; without one the context keeps one for each
         stream it launches on, and gives each call inside a CUDA graph capture one of its own."""
-        self._on_device(o, q, k_pages, v_pages, page_table, lengths, workspace)
-        m = [as_memref(t) for t in (o, q, k_pages, v_pages, page_table, lengths)]
+        call, fn = self._entry("lh_b200_paged_attention")
         if workspace is None:
-            workspace = self._workspace(m[1], m[2])
-        if isinstance(workspace, N.MemRef):
-            mw = workspace
-        else:  # bytes, whatever the element type
-            if not workspace.is_cuda or not workspace.is_contiguous():
-                raise ValueError("the workspace must be a contiguous CUDA tensor")
-            mw = N.memref(workspace.data_ptr(), (workspace.numel() * workspace.element_size() // 4,), (1,), N.LH_F32)
-        N.check(self._lib.lh_b200_paged_attention(self.handle, *map(_ref, m), _ref(mw), float(scale)), self.handle, "lh_b200_paged_attention")
+            ws = self._kept_workspace()
+        elif isinstance(workspace, N.MemRef):
+            ws = workspace
+        else:
+            ws = self._bytes(workspace)
+        rc = call(fn, self.handle.value, self.device, scale, o, q, k_pages, v_pages, page_table, lengths, ws)
+        if rc == N.LH_ERR_NOMEM and workspace is None:
+            ws = self._new_workspace(self.paged_attention_workspace(q, k_pages))
+            rc = call(fn, self.handle.value, self.device, scale, o, q, k_pages, v_pages, page_table, lengths, ws)
+        if rc:
+            N.check(rc, self.handle, "lh_b200_paged_attention")
 
-    def _workspace(self, mq, mk):
+    def _bytes(self, t) -> N.MemRef:
+        """A contiguous tensor of any type as so many bytes of this device."""
+        if not t.is_cuda or t.device.index != self.device or not t.is_contiguous():
+            raise ValueError(f"the workspace must be a contiguous tensor on cuda:{self.device}")
+        return N.memref(t.data_ptr(), (t.numel() * t.element_size() // 4,), (1,), N.LH_F32)
+
+    def _kept_workspace(self) -> N.MemRef:
+        """The workspace of the stream in use; empty (and so refused by the call) if there is none yet,
+        or if the call becomes part of a graph: graphs may run beside one another."""
+        stream, capturing = self._stream_info
+        rc = self._lib.lh_b200_stream_info(self.handle, byref(stream), byref(capturing))
+        if rc:
+            N.check(rc, self.handle, "lh_b200_stream_info")
+        return self._no_workspace if capturing.value else self._workspaces.get(stream.value, self._no_workspace)
+
+    def _new_workspace(self, nbytes: int) -> N.MemRef:
         torch = _torch()
-        need = self.paged_attention_workspace(mq, mk)
-        kept = self.__dict__.setdefault("_workspaces", {})
-        stream = self.stream_handle()
-        ws = kept.get(stream)
-        capturing = torch.cuda.is_current_stream_capturing()
-        if ws is None or ws.numel() < need or capturing:
-            ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{self.device}")
-            # none is given back while the context lives: work still queued, or a captured graph,
-            # may use it
-            self.__dict__.setdefault("_workspaces_held", []).append(ws)
-            if not capturing:
-                kept[stream] = ws
+        t = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+        # none is given back while the context lives: work still queued, or a captured graph, may use it
+        self._workspaces_held.append(t)
+        ws = self._bytes(t)
+        stream, capturing = self._stream_info  # as _kept_workspace left them
+        if not capturing.value:
+            self._workspaces[stream.value] = ws
         return ws
 
     def sample(self, tokens, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, logprobs=None) -> None:
         """One token per row of logits (rows, vocabulary), drawn with ``uniform`` (rows) in [0, 1)
         from what top-k, then top-p, then min-p leave; settings are (rows) tensors or None."""
-        self._on_device(tokens, logits, uniform, temperature, top_k, top_p, min_p, logprobs)
-        m = [as_memref(t) for t in (tokens, logprobs, logits, uniform, temperature, top_k, top_p, min_p)]
-        N.check(self._lib.lh_b200_sample(self.handle, *map(_ref, m)), self.handle, "lh_b200_sample")
+        call, fn = self._entry("lh_b200_sample")
+        rc = call(fn, self.handle.value, self.device, None, tokens, logprobs, logits, uniform, temperature, top_k, top_p, min_p)
+        if rc:
+            N.check(rc, self.handle, "lh_b200_sample")
 
     # -- collectives ---------------------------------------------------------------
     def comm_init(self, unique_id: bytes, rank: int, world: int, nccl_path: str | None = None) -> None:

@@ -232,6 +232,18 @@ extern "C" int lh_b200_ctx_set_stream(lh_ctx_t* ctx, void* cuda_stream, int use_
 
 extern "C" void* lh_b200_ctx_get_stream(lh_ctx_t* ctx) { return ctx ? ctx->stream : nullptr; }
 
+extern "C" int lh_b200_stream_info(lh_ctx_t* ctx, void** stream, int* capturing) {
+  if (!ctx) return LH_ERR_INVALID;
+  if (stream) *stream = ctx->stream;
+  if (capturing) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    DeviceScope scope(ctx->device);
+    LH_CUDA_CHECK(ctx, cudaStreamIsCapturing(ctx->stream, &status));
+    *capturing = status != cudaStreamCaptureStatusNone;
+  }
+  return LH_OK;
+}
+
 extern "C" int lh_b200_sync(lh_ctx_t* ctx) {
   if (!ctx) return LH_ERR_INVALID;
   if (ctx->side_selected) lh_b200_stream_select(ctx, 0);

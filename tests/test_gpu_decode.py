@@ -450,3 +450,90 @@ def test_sample_wide_rows(ctx, vocab):
     check_sample(ctx, logits, u, top_k=[70, 100000, vocab - 1], top_p=[0.9, 0.7, 0.99])
     check_sample(ctx, logits, u, top_p=[0.9, 0.7, 0.99])
     check_sample(ctx, logits, u)
+
+
+# ------------------------------------------------------------------ streams, graphs, workspaces
+def test_captured_calls_follow_the_lengths_and_do_not_share_workspaces(native_lib):
+    """Two graphs of the same context replayed beside one another, while the sequences grow between replays."""
+    from lighthouse_b200.context import CudaContext
+
+    rng = np.random.default_rng(21)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream), CudaContext(0, use_torch_stream=True) as c:
+        sets = []
+        for top in (3000, 2500):
+            k, v, table = cache_of(rng, [top, top // 2, top], 16, 2, 64, "bf16")
+            lens = torch.tensor([5, 0, 17], dtype=torch.int32).cuda()
+            q = randn(rng, 3, 8, 1, 64, dtype="bf16")
+            o = torch.empty_like(q)
+            tab = torch.from_numpy(table).cuda()
+            c.paged_attention(o, q, k, v, tab, lens, 0.125)  # warm: an eager workspace exists
+            stream.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                c.paged_attention(o, q, k, v, tab, lens, 0.125)
+            sets.append((g, o, q, k, v, table, lens, top))
+        other = torch.cuda.Stream()
+        for step in range(4):
+            for g, o, q, k, v, table, lens, top in sets:
+                lens.copy_(torch.tensor([top * step // 3, top * step // 6, min(top, 17 + 900 * step)], dtype=torch.int32))
+                o.fill_(float("nan"))
+            torch.cuda.synchronize()
+            for _ in range(5):
+                sets[0][0].replay()
+                with torch.cuda.stream(other):
+                    sets[1][0].replay()
+            torch.cuda.synchronize()
+            for g, o, q, k, v, table, lens, top in sets:
+                compare_attention(o, q, k, v, table, lens, 0.125)
+
+
+def test_calls_on_another_stream_and_with_a_workspace_of_ones_own(native_lib, own_stream_ctx):
+    rng = np.random.default_rng(22)
+    c = own_stream_ctx  # launches on its own stream, not torch's
+    k, v, table = cache_of(rng, [700, 900], 16, 2, 128, "f16")
+    q = randn(rng, 2, 4, 1, 128, dtype="f16")
+    tab, lens = torch.from_numpy(table).cuda(), torch.tensor([700, 900], dtype=torch.int32).cuda()
+    o = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+    c.paged_attention(o, q, k, v, tab, lens, 0.1)
+    c.sync()
+    compare_attention(o, q, k, v, table, [700, 900], 0.1)
+    n = c.paged_attention_workspace(q, k)
+    ws = torch.full((n + 512,), 0xFF, dtype=torch.uint8, device="cuda")  # whatever it holds before
+    o.fill_(float("nan"))
+    torch.cuda.synchronize()
+    c.paged_attention(o, q, k, v, tab, lens, 0.1, workspace=ws[256:256 + n])
+    c.sync()
+    compare_attention(o, q, k, v, table, [700, 900], 0.1)
+    assert (ws[:256] == 0xFF).all() and (ws[256 + n:] == 0xFF).all()
+
+
+def test_sample_and_append_in_a_graph(native_lib):
+    from lighthouse_b200.context import CudaContext
+
+    rng = np.random.default_rng(23)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream), CudaContext(0, use_torch_stream=True) as c:
+        x, u, t = randn(rng, 5, 40000) * 3, torch.zeros(5, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+        p = torch.full((5,), 0.9, device="cuda")
+        k = randn(rng, 5, 2, 64, dtype="bf16")
+        kp, vp = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+        slots = torch.zeros(5, dtype=torch.int32, device="cuda")
+        c.sample(t, x, u, top_p=p)
+        c.paged_append(None, k, k, kp, vp, slots - 1, theta=0.0)
+        stream.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            c.sample(t, x, u, top_p=p)
+            c.paged_append(None, k, k, kp, vp, slots, theta=0.0)
+        for step in range(3):
+            un = rng.random(5, dtype=np.float32)
+            sn = rng.permutation(64)[:5].astype(np.int32)
+            u.copy_(torch.from_numpy(un))
+            slots.copy_(torch.from_numpy(sn))
+            g.replay()
+            stream.synchronize()
+            want, _ = R.sample(host(x), un, top_p=[np.float32(0.9)] * 5)
+            assert (t.cpu().numpy() == want).all()
+            assert torch.equal(kp.view(64, 2, 64)[torch.from_numpy(sn).cuda().long()], k)
