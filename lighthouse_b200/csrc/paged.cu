@@ -1,5 +1,6 @@
 // The paged key-value cache: writing new rows into it (rotary embedding fused in) and
 // attending over it. Entry points lh_b200_paged_append, lh_b200_paged_attention.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -214,15 +215,26 @@ AppendKernel append_vec_for(int q_dtype, int c_dtype) {
 }
 
 // ---------------------------------------------------------------- attention
-// The general kernel: f32 caches, and 16-bit ones whose rows are not 16-byte aligned. Scores
-// with one key per lane, P V with four head dimensions per lane, both on FFMA; K and V come
-// straight from global memory (a K row is read 16 bytes at a time by its lane, the rest of
-// the sector from L1). Each warp keeps an online softmax of its own over its 32 keys of every
-// tile; the four are joined when the CTA leaves a unit.
-constexpr int SIMT_THREADS = 128;
+// The general kernel, on FFMA: f32 caches, and 16-bit ones whose rows are not 16-byte aligned. For
+// f32 with four query rows to a kv head it needs 512 FFMA and about 250 shared-memory wavefronts
+// per 16 keys of D = 128 (16 KB), half of what an SM has time for while those bytes arrive.
+// A warp fetches 16 keys at a time into a ring of f32 rows (cp.async; or, ASYNC false, loads and
+// conversions of single elements). Scores: a lane has a key and half of its dimensions. P V: a lane
+// has four dimensions (of 64 only half the lanes' worth: the halves take alternate keys).
 constexpr int SIMT_ROWS = 8;
-constexpr int SIMT_TILE = 128;
-constexpr int SIMT_CTAS_PER_SM = 4;
+
+template <int DP>
+struct SimtShape {
+  static constexpr int warps = DP == 256 ? 2 : 4;
+  static constexpr int stages = 3;
+  static constexpr int stage_floats = 2 * TILE * DP;  // K and V rows of 16 keys
+  static constexpr int ctas_per_sm = DP == 64 ? 2 : 1;
+  static constexpr int q_pitch = DP + 8;  // the second half of a row is 4 floats further: no bank in common
+  template <int R>
+  static constexpr int warp_floats() { return stages * stage_floats + R * q_pitch + TILE * R; }
+  template <int R>
+  static constexpr int smem() { return warps * warp_floats<R>() * 4; }
+};
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T x) {
@@ -231,285 +243,383 @@ __device__ __forceinline__ float to_f32(T x) {
   else return __bfloat162float(x);
 }
 
-// Four elements from `d` on; elements at D and beyond read as zero.
-template <typename T, bool VEC>
-__device__ __forceinline__ float4 load4(const T* row, int d, int D) {
-  if constexpr (VEC) {  // D and every offset are multiples of four elements
-    if (d >= D) return make_float4(0.f, 0.f, 0.f, 0.f);
-    if constexpr (std::is_same<T, float>::value) {
-      return *reinterpret_cast<const float4*>(row + d);
-    } else {
-      const uint2 raw = *reinterpret_cast<const uint2*>(row + d);
-      const T* e = reinterpret_cast<const T*>(&raw);
-      return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
-    }
-  } else {
-    return make_float4(d < D ? to_f32(row[d]) : 0.f, d + 1 < D ? to_f32(row[d + 1]) : 0.f, d + 2 < D ? to_f32(row[d + 2]) : 0.f, d + 3 < D ? to_f32(row[d + 3]) : 0.f);
-  }
-}
-
-template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(SIMT_THREADS) paged_simt_kernel(const PagedParams p) {
-  constexpr int DMAX = NV * 128;
-  __shared__ __align__(16) float qs[SIMT_ROWS][DMAX];  // read four at a time
-  __shared__ __align__(16) float obuf[SIMT_ROWS][DMAX];
-  __shared__ float ps[4][SIMT_ROWS][32];
-  __shared__ float wm[4][SIMT_ROWS], wl[4][SIMT_ROWS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+template <typename T, int DP, int R, bool ASYNC>
+__global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas_per_sm) paged_simt_kernel(const PagedParams p) {
+  using S = SimtShape<DP>;
+  constexpr int THREADS = S::warps * 32, CHUNKS = DP / 4, HALF = CHUNKS / 2;
+  constexpr int NV = DP == 256 ? 2 : 1, AT_ONCE = DP == 64 ? 2 : 1;  // P V: vectors of a lane, keys taken at once
+  extern __shared__ __align__(16) float ring_mem[];
+  __shared__ uint32_t there[S::warps][S::stages];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_dependency_trigger();
   int64_t lo, hi;
   TileCursor at;
-  if (!find_stretch<SIMT_THREADS>(p, lo, hi, at)) return;
-  const T* K = static_cast<const T*>(p.k);
-  const T* V = static_cast<const T*>(p.v);
-  while (lo < hi) {
-    const int t0 = at.t;
-    const int t1 = static_cast<int>(at.tiles - t0 <= hi - lo ? at.tiles : t0 + (hi - lo));
-    const int hkv = at.u / p.row_groups, row0 = (at.u % p.row_groups) * SIMT_ROWS;
-    const int nrows = min(SIMT_ROWS, p.rows - row0);
-    for (int i = tid; i < SIMT_ROWS * DMAX; i += SIMT_THREADS) {
-      const int r = i / DMAX, d = i % DMAX;
-      float x = 0.f;
-      if (r < nrows && d < p.D) {
-        const int row = row0 + r;
-        x = to_f32(static_cast<const T*>(p.q)[at.b * p.sqb + row_head(p, hkv, row) * p.sqh + row_token(p, row) * p.sqs + d]) * p.scale_log2;
-      }
-      qs[r][d] = x;
-    }
-    __syncthreads();
-    float m[SIMT_ROWS], l[SIMT_ROWS], acc[SIMT_ROWS][NV * 4];
-    int seen[SIMT_ROWS];  // keys that the row may attend to
-#pragma unroll
-    for (int r = 0; r < SIMT_ROWS; ++r) {
-      seen[r] = r < nrows ? at.len - p.Sq + 1 + row_token(p, row0 + r) : 0;
-      m[r] = -INFINITY;
-      l[r] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV * 4; ++i) acc[r][i] = 0.f;
-    }
-    for (int t = t0; t < t1; ++t) {
-      const int first = t * SIMT_TILE + warp * 32;
-      if (first >= at.len) break;
-      const int j = first + lane;
-      int64_t koff = -1, voff = -1;
-      if (j < at.len) {
-        const int pg = page_of(p, j), slot = j - pg * p.page;
-        const int64_t id = p.table[at.b * p.stb + pg * p.stp];
-        if (id >= 0 && id < p.num_pages) {
-          koff = id * p.skp + slot * p.sks + hkv * p.skh;
-          voff = id * p.svp + slot * p.svs + hkv * p.svh;
+  if (!find_stretch<THREADS>(p, lo, hi, at)) return;
+  float* const ring = ring_mem + warp * S::template warp_floats<R>();
+  float* const qs = ring + S::stages * S::stage_floats;
+  float* const ps = qs + R * S::q_pitch;
+  const T* const K = static_cast<const T*>(p.k);
+  const T* const V = static_cast<const T*>(p.v);
+
+  Fetch f;
+  f.at = at;
+  f.left = hi - lo;
+  f.look_up(p, lane & 15);
+  auto fetch = [&](int stage) {
+    if (f.left <= 0) return;
+    const int key0 = f.at.t * TILE, hkv = f.at.u / p.row_groups;
+    const int j = key0 + (lane & 15);
+    const bool live = j < f.at.len, inside = f.page_id >= 0 && f.page_id < p.num_pages;
+    if (live && !inside) report_bad_index(p.dev_status);
+    const uint32_t mask = __ballot_sync(0xffffffffu, live && inside) & 0xffffu;
+    const int slot = j - page_of(p, j) * p.page;
+    const int64_t ko = live && inside ? f.page_id * p.skp + slot * p.sks + hkv * p.skh : 0;
+    const int64_t vo = live && inside ? f.page_id * p.svp + slot * p.svs + hkv * p.svh : 0;
+    float* const to = ring + stage * S::stage_floats;
+    if (mask) {
+#pragma unroll 8
+      for (int i = 0; i < TILE * CHUNKS / 32; ++i) {
+        const int row = (i * 32 + lane) / CHUNKS, chunk = (i * 32 + lane) % CHUNKS;
+        const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
+        const int d = chunk * 4;
+        const bool get = (mask >> row & 1) && d < p.D;
+        float* const dst = to + row * DP + ((chunk ^ (row & 7)) << 2);
+        if constexpr (ASYNC) {
+          const uint32_t s = smem_u32(dst);
+          cp_async16(s, get ? K + kr + d : K, get ? 16 : 0);
+          cp_async16(s + TILE * DP * 4, get ? V + vr + d : V, get ? 16 : 0);
         } else {
-          report_bad_index(p.dev_status);
+          float k4[4], v4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool one = get && d + e < p.D;
+            k4[e] = one ? to_f32(K[kr + d + e]) : 0.f;
+            v4[e] = one ? to_f32(V[vr + d + e]) : 0.f;
+          }
+          *reinterpret_cast<float4*>(dst) = make_float4(k4[0], k4[1], k4[2], k4[3]);
+          *reinterpret_cast<float4*>(dst + TILE * DP) = make_float4(v4[0], v4[1], v4[2], v4[3]);
         }
       }
-      const bool live = koff >= 0;
-      float s[SIMT_ROWS];
+    }
+    if (lane == 0) there[warp][stage] = mask;
+    f.advance(p);
+    f.look_up(p, lane & 15);
+  };
 #pragma unroll
-      for (int r = 0; r < SIMT_ROWS; ++r) s[r] = 0.f;
-      if (live) {
-#pragma unroll 4
-        for (int d = 0; d < p.D; d += 4) {
-          const float4 kv = load4<T, VEC>(K + koff, d, p.D);
+  for (int s = 0; s < S::stages; ++s) {
+    fetch(s);
+    cp_async_commit();
+  }
+
+  const int key = lane & 15, half = lane >> 4;
+  const int my_chunk = DP == 64 ? lane & 15 : lane;  // P V
+  float m[R], l[R], acc[R][NV * 4];
+  int seen[R];
+  int t0 = at.t, stage = 0;
+  bool fresh = true;
+  for (int64_t left = hi - lo; left > 0; --left) {
+    const int hkv = at.u / p.row_groups, row0 = (at.u % p.row_groups) * R;
+    const int nrows = min(R, p.rows - row0);
+    if (fresh) {
+      fresh = false;
+      t0 = at.t;
+      __syncwarp();
+      for (int i = lane; i < R * DP; i += 32) {
+        const int r = i / DP, d = i % DP;
+        float x = 0.f;
+        if (r < nrows && d < p.D) x = to_f32(static_cast<const T*>(p.q)[at.b * p.sqb + row_head(p, hkv, row0 + r) * p.sqh + row_token(p, row0 + r) * p.sqs + d]) * p.scale_log2;
+        qs[r * S::q_pitch + d + (d >= DP / 2 ? 4 : 0)] = x;
+      }
 #pragma unroll
-          for (int r = 0; r < SIMT_ROWS; ++r) {
-            const float4 qv = *reinterpret_cast<const float4*>(&qs[r][d]);
-            s[r] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[r]))));
-          }
+      for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        seen[r] = r < nrows ? at.len - p.Sq + 1 + row_token(p, row0 + r) : 0;  // keys that the row may attend to
+#pragma unroll
+        for (int i = 0; i < NV * 4; ++i) acc[r][i] = 0.f;
+      }
+    }
+    cp_async_wait<S::stages - 1>();
+    __syncwarp();
+    const uint32_t mask = there[warp][stage];
+    if (mask) {
+      const float* const kt = ring + stage * S::stage_floats;
+      const float* const vt = kt + TILE * DP;
+      const int key0 = at.t * TILE;
+      float s[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r] = 0.f;
+#pragma unroll 8
+      for (int c = 0; c < HALF; ++c) {
+        const float4 kv = *reinterpret_cast<const float4*>(kt + key * DP + (((half * HALF + c) ^ (key & 7)) << 2));
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float4 qv = *reinterpret_cast<const float4*>(qs + r * S::q_pitch + half * (DP / 2 + 4) + c * 4);
+          s[r] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[r]))));
         }
       }
       // keys that only the later of several new tokens may see: masked rows must not meet their V
-      const bool partial = first + 32 > at.len - p.Sq + 1;
+      const bool partial = key0 + TILE > at.len - p.Sq + 1;
+      bool grows = false;
 #pragma unroll
-      for (int r = 0; r < SIMT_ROWS; ++r) {
-        if (!live || j >= seen[r]) s[r] = -INFINITY;
-        float top = s[r];
+      for (int r = 0; r < R; ++r) {
+        s[r] += __shfl_xor_sync(0xffffffffu, s[r], 16);
+        if (!(mask >> key & 1) || key0 + key >= seen[r]) s[r] = -INFINITY;
+        grows |= s[r] > m[r];
+      }
+      // the running maximum is only brought up to date when some key passes it
+      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        top = fmaxf(top, m[r]);
-        const float alpha = exp2_safe(m[r], top), e = exp2_safe(s[r], top);
-        m[r] = top;
-        l[r] = l[r] * alpha + e;
-        ps[warp][r][lane] = e;
+        for (int r = 0; r < R; ++r) {
+          float top = s[r];
 #pragma unroll
-        for (int i = 0; i < NV * 4; ++i) acc[r][i] *= alpha;
+          for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          top = fmaxf(top, m[r]);
+          const float alpha = top == -INFINITY ? 1.f : exp2f(m[r] - top);
+          m[r] = top;
+          l[r] *= alpha;
+#pragma unroll
+          for (int i = 0; i < NV * 4; ++i) acc[r][i] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float e = exp2_safe(s[r], m[r]);
+        l[r] += e;
+        if (half == 0) ps[key * R + r] = e;
       }
       __syncwarp();
 #pragma unroll 4
-      for (int jj = 0; jj < 32; ++jj) {
-        const int64_t off = __shfl_sync(0xffffffffu, voff, jj);
-        if (off < 0) continue;
+      for (int j0 = 0; j0 < TILE; j0 += AT_ONCE) {
+        const int j = AT_ONCE == 2 ? j0 + half : j0;
+        float e[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) e[r] = ps[j * R + r];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const float4 vv = load4<T, VEC>(V + off, i * 128 + lane * 4, p.D);
+          const float4 vv = *reinterpret_cast<const float4*>(vt + j * DP + (((my_chunk + i * 32) ^ (j & 7)) << 2));
 #pragma unroll
-          for (int r = 0; r < SIMT_ROWS; ++r) {
-            const float e = ps[warp][r][jj];
-            if (partial && e == 0.f) continue;
-            acc[r][i * 4 + 0] = fmaf(e, vv.x, acc[r][i * 4 + 0]);
-            acc[r][i * 4 + 1] = fmaf(e, vv.y, acc[r][i * 4 + 1]);
-            acc[r][i * 4 + 2] = fmaf(e, vv.z, acc[r][i * 4 + 2]);
-            acc[r][i * 4 + 3] = fmaf(e, vv.w, acc[r][i * 4 + 3]);
+          for (int r = 0; r < R; ++r) {
+            if (partial && e[r] == 0.f) continue;
+            acc[r][i * 4 + 0] = fmaf(e[r], vv.x, acc[r][i * 4 + 0]);
+            acc[r][i * 4 + 1] = fmaf(e[r], vv.y, acc[r][i * 4 + 1]);
+            acc[r][i * 4 + 2] = fmaf(e[r], vv.z, acc[r][i * 4 + 2]);
+            acc[r][i * 4 + 3] = fmaf(e[r], vv.w, acc[r][i * 4 + 3]);
           }
         }
       }
-      __syncwarp();
     }
-    // join the four warps
+    __syncwarp();
+    if (++at.t == at.tiles || left == 1) {
+      // ---- the warp leaves the unit
+      const int64_t slot = partial_slot<THREADS>(t0, at.t, at.tiles);
 #pragma unroll
-    for (int r = 0; r < SIMT_ROWS; ++r) {
+      for (int r = 0; r < R; ++r) {
 #pragma unroll
-      for (int d = 16; d; d >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
-      if (lane == 0) {
-        wm[warp][r] = m[r];
-        wl[warp][r] = l[r];
-      }
-    }
-    __syncthreads();
-    for (int w = 0; w < 4; ++w) {
-      if (w == warp) {
+        for (int d = 8; d; d >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);  // the two halves hold the same keys
+        if (AT_ONCE == 2) {
 #pragma unroll
-        for (int r = 0; r < SIMT_ROWS; ++r) {
-          const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-          const float f = exp2_safe(m[r], M);
+          for (int i = 0; i < 4; ++i) acc[r][i] += __shfl_xor_sync(0xffffffffu, acc[r][i], 16);
+        }
+        if (r >= nrows) continue;
+        const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];  // a row that sees no key has no weight: zeros
+        const int64_t out = at.b * p.sob + row_head(p, hkv, row0 + r) * p.soh + row_token(p, row0 + r) * p.sos;
+        if (slot >= 0 && lane == 0) p.ml[slot * p.part_rows + r] = make_float2(m[r], l[r]);
 #pragma unroll
-          for (int i = 0; i < NV * 4; ++i) {
-            float* o = &obuf[r][(i / 4) * 128 + lane * 4 + (i & 3)];
-            // a warp without keys adds nothing (its sums are zeros)
-            *o = w == 0 ? acc[r][i] * f : fmaf(acc[r][i], f, *o);
+        for (int i = 0; i < NV; ++i) {
+          const int d = (my_chunk + i * 32) * 4;
+          if (DP == 64 && lane >= 16) break;
+          float4 v = make_float4(acc[r][i * 4], acc[r][i * 4 + 1], acc[r][i * 4 + 2], acc[r][i * 4 + 3]);
+          if (slot < 0) {
+            v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
+            store_o4(p, out, d, v);
+          } else if (d < p.Dp) {
+            *reinterpret_cast<float4*>(p.part + (slot * p.part_rows + r) * p.Dp + d) = v;
           }
         }
       }
-      __syncthreads();
+      fresh = true;
+      if (left > 1) at.next_unit(p);
     }
-    const int64_t slot = partial_slot(t0, t1, at.tiles);
-    for (int i = tid; i < nrows * p.D; i += SIMT_THREADS) {
-      const int r = i / p.D, d = i % p.D, row = row0 + r;
-      const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-      float L = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) L += wl[w][r] * exp2_safe(wm[w][r], M);
-      if (slot < 0) {
-        store_from_f32(p.o, p.o_dtype, at.b * p.sob + row_head(p, hkv, row) * p.soh + row_token(p, row) * p.sos + d, L == 0.f ? 0.f : obuf[r][d] / L);
-      } else {
-        p.part[(slot * p.unit_rows + r) * p.Dp + d] = obuf[r][d];
-        if (d == 0) p.ml[slot * p.unit_rows + r] = make_float2(M, L);
-      }
-    }
-    __syncthreads();
-    lo += t1 - t0;
-    at.t = t1;
-    if (lo < hi && at.t == at.tiles) at.next_unit(p);
+    fetch(stage);
+    cp_async_commit();
+    stage = stage + 1 == S::stages ? 0 : stage + 1;
   }
 }
 
-// Joins the units that several CTAs worked on: block i looks at the border between stretch
-// i - 1 and stretch i, and if it is the first border inside a unit, adds up that unit's parts
-// (8 warps take the parts in turn, a lane holds four head dimensions). The order of the sum is
-// fixed by the stretches. It also writes the zeros of sequences that hold no keys. A programmatic
-// dependent of the kernel above: it is resident and waiting when that one ends.
-constexpr int JOIN_THREADS = 256;
-__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const PagedParams p) {
-  __shared__ float red[JOIN_THREADS / 32];
-  __shared__ float4 sums[JOIN_THREADS / 32][32];
+// Joins the units that several warps worked on: each warp of the join looks at one border between two
+// stretches, and if that is the first border inside a unit, the unit's parts are added up: by the
+// warp itself when they are few, else by its whole block (the warps take the parts in turn, a lane
+// holds four head dimensions). The stretches fix the order of every sum. The kernel also writes the
+// zeros of sequences that hold no keys. It is a programmatic dependent of the kernel above: resident
+// and waiting when that one ends.
+struct JoinWork {
+  int parts;   // 0: nothing to join at this border
+  int b, u;
+  int64_t c0;  // the first part's stretch
+};
+
+__device__ __forceinline__ int64_t join_slot(const JoinWork& w, int c) { return c == 0 ? 2 * w.c0 + 1 : 2 * (w.c0 + c); }
+
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const PagedParams p, int64_t stretches) {
+  __shared__ JoinWork work[JOIN_WARPS];
+  __shared__ float red[JOIN_WARPS];
+  __shared__ float4 sums[JOIN_WARPS][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int ALONE = 8;  // parts that a warp adds up by itself
   grid_dependency_wait();
   if (blockIdx.y == 0) {
     const int64_t per = static_cast<int64_t>(p.Hkv) * p.group * p.Sq * p.D;
     for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
       if (paged_length(p, b)) continue;
-      for (int64_t i = tid; i < per; i += JOIN_THREADS) {
+      for (int64_t i = tid; i < per; i += JOIN_WARPS * 32) {
         const int d = static_cast<int>(i % p.D);
         const int64_t rest = i / p.D;
         store_from_f32(p.o, p.o_dtype, b * p.sob + (rest / p.Sq) * p.soh + (rest % p.Sq) * p.sos + d, 0.f);
       }
     }
   }
-  if (blockIdx.x == 0) return;
-  const int4 here = p.first[blockIdx.x];
-  if (here.x < 0 || here.z == 0) return;  // no stretch, or one that begins with its unit
-  const int64_t total = *p.total;
-  const int64_t n = total < gridDim.x ? total : gridDim.x;
-  const int64_t lo = stretch_begin(total, n, blockIdx.x);
-  const int64_t begin = lo - here.z;
-  if (stretch_begin(total, n, blockIdx.x - 1) > begin) return;  // an earlier block has this unit
-  const int len = paged_length(p, here.x);
-  const int64_t end = begin + paged_tiles(p, len);
-  const int64_t c0 = blockIdx.x - 1;
-  const int parts = static_cast<int>(stretch_owner(total, n, end - 1) - c0 + 1);
-  auto slot_of = [&](int c) { return c == 0 ? 2 * c0 + 1 : 2 * (c0 + c); };
-  const int hkv = here.y / p.row_groups, row0 = (here.y % p.row_groups) * p.unit_rows;
-  const int nrows = min(p.unit_rows, p.rows - row0);
-  for (int r = blockIdx.y; r < nrows; r += gridDim.y) {
-    float M = -INFINITY;
-    for (int c = tid; c < parts; c += JOIN_THREADS) M = fmaxf(M, p.ml[slot_of(c) * p.unit_rows + r].x);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-    if (lane == 0) red[warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < JOIN_THREADS / 32; ++w) M = fmaxf(M, red[w]);
-    const int row = row0 + r;
-    const int64_t out = here.x * p.sob + row_head(p, hkv, row) * p.soh + row_token(p, row) * p.sos;
-    for (int d0 = 0; d0 < p.Dp; d0 += 128) {
-      const int d = d0 + lane * 4;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-      float L = 0.f;
-      for (int c = warp; c < parts; c += JOIN_THREADS / 32) {
-        const int64_t at = slot_of(c) * p.unit_rows + r;
-        const float2 ml = p.ml[at];
-        const float f = exp2_safe(ml.x, M);
-        L = fmaf(ml.y, f, L);
-        if (d < p.Dp) {
-          const float4 x = *reinterpret_cast<const float4*>(p.part + at * p.Dp + d);
-          a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
-        }
-      }
-      __syncthreads();
-      sums[warp][lane] = a;
-      if (lane == 0) red[warp] = L;
-      __syncthreads();
-      if (warp == 0) {
-        L = 0.f;
-        a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < JOIN_THREADS / 32; ++w) {
-          const float4 x = sums[w][lane];
-          a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-          L += red[w];
-        }
-        // a row that sees no key has no weight at all: zeros
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        if (d < p.D) store_from_f32(p.o, p.o_dtype, out + d, a.x * inv);
-        if (d + 1 < p.D) store_from_f32(p.o, p.o_dtype, out + d + 1, a.y * inv);
-        if (d + 2 < p.D) store_from_f32(p.o, p.o_dtype, out + d + 2, a.z * inv);
-        if (d + 3 < p.D) store_from_f32(p.o, p.o_dtype, out + d + 3, a.w * inv);
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * JOIN_WARPS + warp;
+  JoinWork w = {0, 0, 0, 0};
+  if (i > 0 && i < stretches) {
+    const int4 here = p.first[i];
+    if (here.x >= 0 && here.z > 0) {  // a stretch that begins inside its unit
+      const int64_t total = *p.total;
+      const int64_t n = total < stretches ? total : stretches;
+      const int64_t begin = stretch_begin(total, n, i) - here.z;
+      if (stretch_begin(total, n, i - 1) <= begin) {  // no earlier border lies in this unit
+        const int64_t end = begin + paged_tiles(paged_length(p, here.x));
+        w.c0 = i - 1;
+        w.parts = static_cast<int>(stretch_owner(total, n, end - 1) - w.c0 + 1);
+        w.b = here.x;
+        w.u = here.y;
       }
     }
-    __syncthreads();
+  }
+  if (lane == 0) work[warp] = w;
+  if (w.parts && w.parts <= ALONE) {
+    const int hkv = w.u / p.row_groups, row0 = (w.u % p.row_groups) * p.unit_rows;
+    const int nrows = min(p.unit_rows, p.rows - row0);
+    for (int r = blockIdx.y; r < nrows; r += gridDim.y) {
+      const float2 mine = lane < w.parts ? p.ml[join_slot(w, lane) * p.part_rows + r] : make_float2(-INFINITY, 0.f);
+      float M = mine.x;
+#pragma unroll
+      for (int d = 4; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+      M = __shfl_sync(0xffffffffu, M, 0);
+      const float scale = exp2_safe(mine.x, M), weight = mine.y * scale;
+      float L = 0.f;
+#pragma unroll
+      for (int c = 0; c < ALONE; ++c) L += __shfl_sync(0xffffffffu, weight, c);
+      const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key has no weight: zeros
+      const int row = row0 + r;
+      const int64_t out = w.b * p.sob + row_head(p, hkv, row) * p.soh + row_token(p, row) * p.sos;
+      for (int d0 = 0; d0 < p.Dp; d0 += 128) {
+        const int d = d0 + lane * 4;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < ALONE; ++c) {
+          const float k = __shfl_sync(0xffffffffu, scale, c);
+          if (c < w.parts && d < p.Dp) {
+            const float4 x = *reinterpret_cast<const float4*>(p.part + (join_slot(w, c) * p.part_rows + r) * p.Dp + d);
+            a.x = fmaf(x.x, k, a.x); a.y = fmaf(x.y, k, a.y); a.z = fmaf(x.z, k, a.z); a.w = fmaf(x.w, k, a.w);
+          }
+        }
+        store_o4(p, out, d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+      }
+    }
+  }
+  __syncthreads();
+  for (int q = 0; q < JOIN_WARPS; ++q) {
+    w = work[q];
+    if (w.parts <= ALONE) continue;
+    const int hkv = w.u / p.row_groups, row0 = (w.u % p.row_groups) * p.unit_rows;
+    const int nrows = min(p.unit_rows, p.rows - row0);
+    for (int r = blockIdx.y; r < nrows; r += gridDim.y) {
+      float M = -INFINITY;
+      for (int c = tid; c < w.parts; c += JOIN_WARPS * 32) M = fmaxf(M, p.ml[join_slot(w, c) * p.part_rows + r].x);
+#pragma unroll
+      for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+      if (lane == 0) red[warp] = M;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < JOIN_WARPS; ++k) M = fmaxf(M, red[k]);
+      const int row = row0 + r;
+      const int64_t out = w.b * p.sob + row_head(p, hkv, row) * p.soh + row_token(p, row) * p.sos;
+      for (int d0 = 0; d0 < p.Dp; d0 += 128) {
+        const int d = d0 + lane * 4;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
+#pragma unroll 8
+        for (int c = warp; c < w.parts; c += JOIN_WARPS) {
+          const int64_t from = join_slot(w, c) * p.part_rows + r;
+          const float2 ml = p.ml[from];
+          const float k = exp2_safe(ml.x, M);
+          L = fmaf(ml.y, k, L);
+          if (d < p.Dp) {
+            const float4 x = *reinterpret_cast<const float4*>(p.part + from * p.Dp + d);
+            a.x = fmaf(x.x, k, a.x); a.y = fmaf(x.y, k, a.y); a.z = fmaf(x.z, k, a.z); a.w = fmaf(x.w, k, a.w);
+          }
+        }
+        __syncthreads();
+        sums[warp][lane] = a;
+        if (lane == 0) red[warp] = L;
+        __syncthreads();
+        if (warp == 0) {
+          L = 0.f;
+          a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < JOIN_WARPS; ++k) {
+            const float4 x = sums[k][lane];
+            a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+            L += red[k];
+          }
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          store_o4(p, out, d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+        }
+      }
+      __syncthreads();
+    }
   }
 }
 
-int join_launch(lh_ctx* ctx, const PagedParams& p, int ctas) {
+int join_launch(lh_ctx* ctx, const PagedParams& p, int64_t stretches) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(p.rows < p.unit_rows ? p.rows : p.unit_rows));
-  cfg.blockDim = dim3(JOIN_THREADS);
+  // rows side by side: a unit split over the whole GPU has many parts to each row
+  cfg.gridDim = dim3(static_cast<unsigned>((stretches + JOIN_WARPS - 1) / JOIN_WARPS), static_cast<unsigned>(p.part_rows < 8 ? p.part_rows : 8));
+  cfg.blockDim = dim3(JOIN_WARPS * 32);
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  LH_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, paged_join_kernel, p));
+  LH_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, paged_join_kernel, p, stretches));
   LH_CHECK_LAUNCH(ctx, "paged_join_kernel");
   return LH_OK;
 }
 
-typedef void (*PagedKernel)(const PagedParams);
-template <typename T>
-PagedKernel simt_kernel_for(int D, bool vec) {
-  if (D <= 128) return vec ? paged_simt_kernel<T, 1, true> : paged_simt_kernel<T, 1, false>;
-  return vec ? paged_simt_kernel<T, 2, true> : paged_simt_kernel<T, 2, false>;
+int simt_unit_rows(int64_t rows) { return rows <= 2 ? 2 : rows <= 4 ? 4 : SIMT_ROWS; }
+int simt_stretches(const lh_ctx* ctx, int D) {
+  return ctx->sm_count * (D <= 64 ? SimtShape<64>::warps * SimtShape<64>::ctas_per_sm : D <= 128 ? SimtShape<128>::warps * SimtShape<128>::ctas_per_sm : SimtShape<256>::warps * SimtShape<256>::ctas_per_sm);
+}
+
+template <typename T, int DP, int R, bool ASYNC>
+int simt_launch(lh_ctx* ctx, const PagedParams& p, int stretches) {
+  constexpr int smem = SimtShape<DP>::template smem<R>();
+  auto* kernel = paged_simt_kernel<T, DP, R, ASYNC>;
+  LH_CUDA_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<static_cast<unsigned>(stretches / SimtShape<DP>::warps), SimtShape<DP>::warps * 32, smem, ctx->stream>>>(p);
+  LH_CHECK_LAUNCH(ctx, "paged_simt_kernel");
+  return LH_OK;
+}
+template <typename T, int DP, bool ASYNC>
+int simt_launch_rows(lh_ctx* ctx, const PagedParams& p, int stretches) {
+  return p.unit_rows == 2 ? simt_launch<T, DP, 2, ASYNC>(ctx, p, stretches) : p.unit_rows == 4 ? simt_launch<T, DP, 4, ASYNC>(ctx, p, stretches) : simt_launch<T, DP, SIMT_ROWS, ASYNC>(ctx, p, stretches);
+}
+template <typename T, bool ASYNC>
+int simt_launch_size(lh_ctx* ctx, const PagedParams& p, int stretches) {
+  return p.D <= 64 ? simt_launch_rows<T, 64, ASYNC>(ctx, p, stretches) : p.D <= 128 ? simt_launch_rows<T, 128, ASYNC>(ctx, p, stretches) : simt_launch_rows<T, 256, ASYNC>(ctx, p, stretches);
 }
 
 bool aligned_view(const lh_memref_t* m, int elems) {
@@ -537,13 +647,13 @@ bool sane_extents(const lh_memref_t* m) {
 struct Workspace {
   size_t first, ml, part, bytes;
 };
-Workspace workspace_for(int64_t ctas, int unit_rows, int Dp) {
+Workspace workspace_for(int64_t stretches, int64_t rows, int Dp) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   Workspace w;
   w.first = 256;  // the tile count comes first
-  w.ml = w.first + up(ctas * sizeof(int4));
-  w.part = w.ml + up(2 * ctas * unit_rows * sizeof(float2));
-  w.bytes = w.part + up(2 * ctas * static_cast<size_t>(unit_rows) * Dp * sizeof(float));
+  w.ml = w.first + up(stretches * sizeof(int4));
+  w.part = w.ml + up(2 * stretches * rows * sizeof(float2));
+  w.bytes = w.part + up(2 * stretches * static_cast<size_t>(rows) * Dp * sizeof(float));
   return w;
 }
 
@@ -573,8 +683,6 @@ int check_attention(lh_ctx* ctx, const lh_memref_t* o, const lh_memref_t* q, con
   if (q->shape[1] * q->shape[2] > 0x7fffffffll || q->shape[2] > 0x3fffffffll) return set_error(ctx, LH_ERR_UNSUPPORTED, "paged_attention: too many query rows");
   return LH_OK;
 }
-
-int64_t simt_ctas(const lh_ctx* ctx) { return static_cast<int64_t>(ctx->sm_count) * SIMT_CTAS_PER_SM; }
 
 }  // namespace
 }  // namespace lh
@@ -655,12 +763,11 @@ extern "C" int lh_b200_paged_attention_workspace(lh_ctx_t* ctx, const lh_memref_
   if (!ctx) return LH_ERR_INVALID;
   if (!q || !k_pages || !bytes || q->rank != 4 || k_pages->rank != 4 || k_pages->shape[2] < 1) return set_error(ctx, LH_ERR_INVALID, "paged_attention_workspace: q (B, Hq, S, D), k_pages (pages, page_size, Hkv, D) and bytes are required");
   // enough for whichever kernel the operands' alignment selects
-  const int Dp = static_cast<int>((q->shape[3] + 3) / 4 * 4);
+  const int Dp = static_cast<int>((q->shape[3] + 3) / 4 * 4), D = q->shape[3] > 256 ? 256 : static_cast<int>(q->shape[3]);
   const int64_t rows = q->shape[1] / k_pages->shape[2] * q->shape[2];
-  const size_t simt = workspace_for(simt_ctas(ctx), SIMT_ROWS, Dp).bytes;
-  const int D = q->shape[3] > 256 ? 256 : static_cast<int>(q->shape[3]);
-  const size_t mma = workspace_for(paged_mma_ctas(ctx, D), paged_mma_unit_rows(rows, D), Dp).bytes;
-  *bytes = simt > mma ? simt : mma;
+  const size_t simt = workspace_for(simt_stretches(ctx, D), std::min<int64_t>(rows, simt_unit_rows(rows)), Dp).bytes;
+  const size_t mma = workspace_for(paged_mma_stretches(ctx, D), std::min<int64_t>(rows, paged_mma_unit_rows(rows, D)), Dp).bytes;
+  *bytes = std::max(simt, mma);
   return LH_OK;
 }
 
@@ -699,26 +806,21 @@ extern "C" int lh_b200_paged_attention(lh_ctx_t* ctx, const lh_memref_t* o, cons
   p.Dp = (p.D + 3) / 4 * 4;
   p.dev_status = ctx->dev_status;
   const bool mma = paged_mma_supported(k_pages, v_pages);
-  p.unit_rows = mma ? paged_mma_unit_rows(p.rows, p.D) : SIMT_ROWS;
-  p.tile = SIMT_TILE;
-  const int ctas = static_cast<int>(mma ? paged_mma_ctas(ctx, p.D) : simt_ctas(ctx));
+  p.unit_rows = mma ? paged_mma_unit_rows(p.rows, p.D) : simt_unit_rows(p.rows);
+  p.part_rows = std::min(p.rows, p.unit_rows);
+  const int stretches = mma ? paged_mma_stretches(ctx, p.D) : simt_stretches(ctx, p.D);
+  p.o_vec = p.D % 4 == 0 && aligned_view(o, 4);
   p.row_groups = (p.rows + p.unit_rows - 1) / p.unit_rows;
   if (static_cast<int64_t>(p.Hkv) * p.row_groups > 0x7fffffffll) return set_error(ctx, LH_ERR_UNSUPPORTED, "paged_attention: too many query rows");
-  const Workspace w = workspace_for(ctas, p.unit_rows, p.Dp);
+  const Workspace w = workspace_for(stretches, p.part_rows, p.Dp);
   char* base = data_ptr(workspace);
   p.total = reinterpret_cast<int64_t*>(base);
   p.first = reinterpret_cast<int4*>(base + w.first);
   p.ml = reinterpret_cast<float2*>(base + w.ml);
   p.part = reinterpret_cast<float*>(base + w.part);
   DeviceScope scope(ctx->device);
-  if (mma) {
-    rc = paged_mma_launch(ctx, p, q->dtype, ctas);
-    if (rc) return rc;
-    return join_launch(ctx, p, ctas);
-  }
-  const bool vec = p.D % 4 == 0 && aligned_view(k_pages, 4) && aligned_view(v_pages, 4);
-  PagedKernel kernel = q->dtype == LH_F32 ? simt_kernel_for<float>(p.D, vec) : q->dtype == LH_BF16 ? simt_kernel_for<__nv_bfloat16>(p.D, vec) : simt_kernel_for<__half>(p.D, vec);
-  kernel<<<static_cast<unsigned>(ctas), SIMT_THREADS, 0, ctx->stream>>>(p);
-  LH_CHECK_LAUNCH(ctx, "paged_simt_kernel");
-  return join_launch(ctx, p, ctas);
+  if (mma) rc = paged_mma_launch(ctx, p, q->dtype, stretches);
+  else if (q->dtype == LH_F32) rc = p.D % 4 == 0 && aligned_view(k_pages, 4) && aligned_view(v_pages, 4) ? simt_launch_size<float, true>(ctx, p, stretches) : simt_launch_size<float, false>(ctx, p, stretches);
+  else rc = q->dtype == LH_BF16 ? simt_launch_size<__nv_bfloat16, false>(ctx, p, stretches) : simt_launch_size<__half, false>(ctx, p, stretches);
+  return rc ? rc : join_launch(ctx, p, stretches);
 }

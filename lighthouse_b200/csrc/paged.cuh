@@ -1,9 +1,10 @@
 // Attention of new tokens over a paged key-value cache: what its kernels share. The keys of a
-// sequence are cut into tiles; all tiles of a call form one line (sequence, then unit, then
-// tile; a unit is a kv head and a group of its query rows), and every CTA takes an equal
-// stretch of that line. The lengths live on the device, so each CTA works out its stretch
-// itself: a call needs no knowledge of them on the host, replays as a graph while sequences
-// grow, and a ragged batch is balanced to within one tile.
+// sequence are cut into tiles of 16; all tiles of a call form one line (sequence, then unit, then
+// tile; a unit is a kv head and a group of its query rows), and every WARP takes an equal stretch
+// of that line, with loads, online softmax and results of its own. The lengths live on the
+// device, so each CTA works out its warps' stretches itself: a call needs no knowledge of them on
+// the host, replays as a graph while sequences grow, and a ragged batch is balanced to within one
+// tile. Where a stretch ends inside a unit, the warp leaves a partial result to the join kernel.
 #pragma once
 #include "common.cuh"
 #include "epilogue.cuh"
@@ -26,28 +27,30 @@ struct PagedParams {
   int page, page_shift;   // page_shift < 0: the page size is no power of two
   int max_keys;           // table columns x page size
   int rows, unit_rows, row_groups;  // query rows of a kv head (tokens x group), rows of a unit, units of a kv head
-  int tile;               // keys of a tile
-  int o_dtype;
+  int o_dtype, o_vec;     // o_vec: four elements of a row of o can be stored at once
   float scale_log2;       // softmax scale x log2(e): scores are kept as powers of two
   // workspace
   int64_t* total;         // tiles of the whole call
-  int4* first;            // per CTA: (sequence, unit, tile) its stretch starts at; x < 0: no stretch
+  int4* first;            // per stretch: (sequence, unit, tile) it starts at; x < 0: it has none
   float2* ml;             // per partial row: running maximum and sum
   float* part;            // per partial row: Dp floats, not yet divided by the sum
-  int Dp;
+  int Dp, part_rows;      // floats of a partial row, rows of a partial result
   int* dev_status;
 };
 
-// CTA i of n owns tiles [total * i / n, total * (i + 1) / n); no stretch is empty because n <= total.
+constexpr int TILE = 16;  // keys of a tile
+constexpr int JOIN_WARPS = 8;
+
+// Stretch i of n is tiles [total * i / n, total * (i + 1) / n); none is empty because n <= total.
 __host__ __device__ __forceinline__ int64_t stretch_begin(int64_t total, int64_t n, int64_t i) { return total * i / n; }
-// The CTA that owns tile x: the last i with total * i / n < x + 1.
+// The stretch that has tile x: the last i with total * i / n < x + 1.
 __host__ __device__ __forceinline__ int64_t stretch_owner(int64_t total, int64_t n, int64_t x) { return ((x + 1) * n - 1) / total; }
 
 __device__ __forceinline__ int paged_length(const PagedParams& p, int b) {
   const int len = p.lengths[b * p.slen];
   return len < 0 ? 0 : len > p.max_keys ? p.max_keys : len;
 }
-__device__ __forceinline__ int paged_tiles(const PagedParams& p, int len) { return (len + p.tile - 1) / p.tile; }
+__device__ __forceinline__ int paged_tiles(int len) { return (len + TILE - 1) / TILE; }
 
 __device__ __forceinline__ int page_of(const PagedParams& p, int j) { return p.page_shift >= 0 ? j >> p.page_shift : j / p.page; }
 
@@ -57,11 +60,11 @@ struct TileCursor {
   __device__ __forceinline__ void seek(const PagedParams& p, int b_, int64_t within) {
     b = b_;
     len = paged_length(p, b);
-    tiles = paged_tiles(p, len);
+    tiles = paged_tiles(len);
     u = static_cast<int>(within / tiles);
     t = static_cast<int>(within % tiles);
   }
-  // Only called while tiles of this CTA's stretch remain, so the next sequence exists.
+  // Only called while tiles of this warp's stretch remain, so the next sequence exists.
   __device__ __forceinline__ void next_unit(const PagedParams& p) {
     t = 0;
     if (++u < p.Hkv * p.row_groups) return;
@@ -70,17 +73,18 @@ struct TileCursor {
       ++b;
       len = paged_length(p, b);
     } while (len == 0);
-    tiles = paged_tiles(p, len);
+    tiles = paged_tiles(len);
   }
 };
 
-// Every thread of the block gets this CTA's stretch [lo, hi) and where it starts.
-// Prefix sum over the sequences: each thread adds up a run of them, the block scans the runs.
+// Each warp gets its stretch [lo, hi) and where it starts; false for warps without one. Prefix sum over
+// the sequences: each thread adds up a run of them, the block scans the runs. All threads call it.
 template <int NT>
 __device__ __forceinline__ bool find_stretch(const PagedParams& p, int64_t& lo, int64_t& hi, TileCursor& at) {
-  __shared__ int64_t warp_sum[NT / 32];
-  __shared__ int64_t start_base;
-  __shared__ int start_b;
+  constexpr int W = NT / 32;
+  __shared__ int64_t warp_sum[W];
+  __shared__ int64_t start_base[W];
+  __shared__ int start_b[W];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int units = p.Hkv * p.row_groups;
   const int run = (p.B + NT - 1) / NT;
@@ -91,7 +95,7 @@ __device__ __forceinline__ bool find_stretch(const PagedParams& p, int64_t& lo, 
   for (int b = b0; b < b1; ++b) {
     const int raw = p.lengths[b * p.slen];
     if (blockIdx.x == 0 && (raw < 0 || raw > p.max_keys)) report_bad_index(p.dev_status);
-    mine += static_cast<int64_t>(paged_tiles(p, paged_length(p, b))) * units;
+    mine += static_cast<int64_t>(paged_tiles(paged_length(p, b))) * units;
   }
   int64_t incl = mine;
 #pragma unroll
@@ -103,47 +107,99 @@ __device__ __forceinline__ bool find_stretch(const PagedParams& p, int64_t& lo, 
   __syncthreads();
   int64_t before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < NT / 32; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
-  const int64_t n = total < gridDim.x ? total : gridDim.x;
+  const int64_t stretches = static_cast<int64_t>(gridDim.x) * W;
+  const int64_t n = total < stretches ? total : stretches;
   if (blockIdx.x == 0 && tid == 0) *p.total = total;
-  if (blockIdx.x >= n) {
-    if (tid == 0) p.first[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    return false;
-  }
-  lo = stretch_begin(total, n, blockIdx.x);
-  hi = stretch_begin(total, n, blockIdx.x + 1);
-  int64_t base = before + incl - mine;
-  if (lo >= base && lo < base + mine) {
+  const int64_t base = before + incl - mine;
+  for (int w = 0; w < W; ++w) {
+    const int64_t s = static_cast<int64_t>(blockIdx.x) * W + w;
+    if (s >= n) break;
+    const int64_t begin = stretch_begin(total, n, s);
+    if (begin < base || begin >= base + mine) continue;
+    int64_t at_base = base;
     for (int b = b0; b < b1; ++b) {
-      const int64_t here = static_cast<int64_t>(paged_tiles(p, paged_length(p, b))) * units;
-      if (lo < base + here) {
-        start_b = b;
-        start_base = base;
+      const int64_t here = static_cast<int64_t>(paged_tiles(paged_length(p, b))) * units;
+      if (begin < at_base + here) {
+        start_b[w] = b;
+        start_base[w] = at_base;
         break;
       }
-      base += here;
+      at_base += here;
     }
   }
   __syncthreads();
-  at.seek(p, start_b, lo - start_base);
-  if (tid == 0) p.first[blockIdx.x] = make_int4(at.b, at.u, at.t, 0);
+  const int64_t s = static_cast<int64_t>(blockIdx.x) * W + warp;
+  if (s >= n) {
+    if (lane == 0) p.first[s] = make_int4(-1, 0, 0, 0);
+    return false;
+  }
+  lo = stretch_begin(total, n, s);
+  hi = stretch_begin(total, n, s + 1);
+  at.seek(p, start_b[warp], lo - start_base[warp]);
+  if (lane == 0) p.first[s] = make_int4(at.b, at.u, at.t, 0);
   return true;
 }
 
-// Where this CTA's part of unit (tiles t0 .. t1 of `tiles`) goes: -1 when it is the whole unit,
-// else one of the CTA's two partial slots (the stretch's first unit may begin before it, its
-// last may end after it).
+// Where a warp's part of a unit (tiles t0 .. t1 of `tiles`) goes: -1 when it is the whole unit, else
+// one of the stretch's two partial slots (its first unit may begin before it, its last may end
+// after it).
+template <int NT>
 __device__ __forceinline__ int64_t partial_slot(int t0, int t1, int tiles) {
   if (t0 == 0 && t1 == tiles) return -1;
-  return 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
+  return 2 * (static_cast<int64_t>(blockIdx.x) * (NT / 32) + (threadIdx.x >> 5)) + (t0 == 0 ? 1 : 0);
 }
 
 // 2^(x - m) against a running maximum m. Before any key counted (m = -inf) a score is either
 // -inf, of no weight, or NaN, which stays one.
 __device__ __forceinline__ float exp2_safe(float x, float m) { return m == -INFINITY ? (x == -INFINITY ? 0.f : x) : exp2f(x - m); }
+
+// Four head dimensions from d on of a row of o (those below D).
+__device__ __forceinline__ void store_o4(const PagedParams& p, int64_t row, int d, float4 v) {
+  if (p.o_vec) {  // D is a multiple of four
+    if (d >= p.D) return;
+    if (p.o_dtype == LH_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(p.o) + row + d) = v;
+    } else if (p.o_dtype == LH_BF16) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.o) + row + d) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+      const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(static_cast<__half*>(p.o) + row + d) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+    return;
+  }
+  if (d < p.D) store_from_f32(p.o, p.o_dtype, row + d, v.x);
+  if (d + 1 < p.D) store_from_f32(p.o, p.o_dtype, row + d + 1, v.y);
+  if (d + 2 < p.D) store_from_f32(p.o, p.o_dtype, row + d + 2, v.z);
+  if (d + 3 < p.D) store_from_f32(p.o, p.o_dtype, row + d + 3, v.w);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// What the side of a warp that fetches knows: the next tile to fetch and, one step ahead of its use,
+// the page that holds this lane's key of it.
+struct Fetch {
+  TileCursor at;
+  int64_t left;  // tiles still to fetch
+  int page_id;
+  __device__ __forceinline__ void look_up(const PagedParams& p, int key_in_tile) {
+    const int j = at.t * TILE + key_in_tile;
+    page_id = left > 0 && j < at.len ? p.table[at.b * p.stb + page_of(p, j) * p.stp] : -1;
+  }
+  __device__ __forceinline__ void advance(const PagedParams& p) {
+    --left;
+    if (++at.t == at.tiles && left > 0) at.next_unit(p);
+  }
+};
 
 // Query row r of unit u: which token and head it is.
 __device__ __forceinline__ int row_token(const PagedParams& p, int row) { return row / p.group; }
@@ -152,7 +208,7 @@ __device__ __forceinline__ int row_head(const PagedParams& p, int hkv, int row) 
 // The tensor-core kernel (paged_mma.cu).
 bool paged_mma_supported(const lh_memref_t* k, const lh_memref_t* v);
 int paged_mma_unit_rows(int64_t rows, int D);
-int paged_mma_ctas(const lh_ctx* ctx, int D);
-int paged_mma_launch(lh_ctx* ctx, PagedParams& p, int dtype, int ctas);
+int paged_mma_stretches(const lh_ctx* ctx, int D);
+int paged_mma_launch(lh_ctx* ctx, const PagedParams& p, int dtype, int stretches);
 
 }  // namespace lh

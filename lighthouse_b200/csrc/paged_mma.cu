@@ -12,10 +12,10 @@
 // first product with keys along the rows; movmatrix turns its 8 x 8 blocks into the second
 // product's operand in registers.
 //
-// Each warp runs by itself: it takes 16 of the tile's 64 keys, fetches them with cp.async into
-// its own ring of stages and keeps its own online softmax, so the main loop has no block-wide
-// barrier. The four warps are joined when the CTA leaves a unit; the ring is already being
-// filled for the next unit meanwhile.
+// Each warp runs by itself, on its own stretch of tiles: it fetches 16 keys at a time with cp.async
+// into a ring of its own and keeps its own online softmax, so nothing in the kernel after its
+// first microsecond waits for another warp. At the end of a unit the results are turned to rows in
+// the stage just used, while the ring is already being filled for the next unit.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -24,22 +24,14 @@ namespace lh {
 namespace {
 
 constexpr int THREADS = 128;
-constexpr int TILE = 64;  // keys of a tile, 16 per warp
-constexpr int SUB = 16;
+constexpr int SUB = TILE;
 
 template <int DP>
 struct Shape {
-  static constexpr int stage_bytes = 2 * SUB * DP * 2;  // K and V rows of one warp's 16 keys
+  static constexpr int stage_bytes = 2 * SUB * DP * 2;  // K and V rows of 16 keys
   static constexpr int stages = DP == 64 ? 6 : 3;
   static constexpr int ctas_per_sm = DP == 256 ? 1 : 2;
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -82,23 +74,13 @@ __device__ __forceinline__ float bits_to_f32(uint32_t bits16) {
   else return __uint_as_float(bits16 << 16);
 }
 
-// What the ring's producer side knows: the next tile to fetch and, one step ahead of its use,
-// the page that holds this lane's key of it.
-struct Fetch {
-  TileCursor at;
-  int64_t left;  // tiles still to fetch
-  int page_id;
-};
-
 template <typename T, int DP, int NT, bool WHOLE_PAGE>
 __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_kernel(const PagedParams p) {
   constexpr int STAGES = Shape<DP>::stages, STAGE_BYTES = Shape<DP>::stage_bytes, V_OFF = STAGE_BYTES / 2;
   constexpr int CHUNKS = DP / 8;             // 16-byte chunks of a row
   constexpr int ROWS_AT_ONCE = 32 / CHUNKS;  // rows that one cp.async per lane covers
   constexpr int KSTEPS = DP / 16;
-  constexpr int OB = DP + 4;  // row pitch of the join buffer: its 8 x 4 lanes hit 32 banks
   extern __shared__ __align__(128) char smem[];
-  __shared__ float wm[4][NT * 8], wl[4][NT * 8];
   __shared__ uint32_t there[4][STAGES];  // which of a stage's 16 keys exist
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -109,7 +91,6 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
 
   const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE_BYTES;
   char* const ring_ptr = smem + warp * STAGES * STAGE_BYTES;
-  float* const obuf = reinterpret_cast<float*>(smem + 4 * STAGES * STAGE_BYTES);
   const T* const K = static_cast<const T*>(p.k);
   const T* const V = static_cast<const T*>(p.v);
 
@@ -119,15 +100,11 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
   Fetch f;
   f.at = at;
   f.left = hi - lo;
-  // -1: no such key; INT_MIN would do as well, any id outside the pool is not fetched
-  auto look_up = [&]() {
-    const int j = f.at.t * TILE + warp * SUB + (WHOLE_PAGE ? 0 : lane & 15);
-    f.page_id = f.left > 0 && j < f.at.len ? p.table[f.at.b * p.stb + page_of(p, j) * p.stp] : -1;
-  };
-  look_up();
+  const int my_key = WHOLE_PAGE ? 0 : lane & 15;  // WHOLE_PAGE: a tile lies within one page
+  f.look_up(p, my_key);
   auto fetch = [&](int stage) {
     if (f.left <= 0) return;
-    const int key0 = f.at.t * TILE + warp * SUB;
+    const int key0 = f.at.t * TILE;
     const int hkv = f.at.u / p.row_groups;
     const bool inside = f.page_id >= 0 && f.page_id < p.num_pages;
     const uint32_t base = ring + stage * STAGE_BYTES;
@@ -170,9 +147,8 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
       }
     }
     if (lane == 0) there[warp][stage] = mask;
-    --f.left;
-    if (++f.at.t == f.at.tiles && f.left > 0) f.at.next_unit(p);
-    look_up();
+    f.advance(p);
+    f.look_up(p, my_key);
   };
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) {
@@ -228,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
     const uint32_t mask = there[warp][stage];
     if (mask) {
       const uint32_t base = ring + stage * STAGE_BYTES;
-      const int key0 = at.t * TILE + warp * SUB;
+      const int key0 = at.t * TILE;
       float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -335,68 +311,63 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
       }
     }
     __syncwarp();
+    if (++at.t == at.tiles || left == 1) {
+      // ---- the warp leaves the unit. The stage just used takes two n tiles of results as rows of f32;
+      // dimensions are swizzled by the row so that neither side meets in a bank.
+      float* const buf = reinterpret_cast<float*>(ring_ptr + stage * STAGE_BYTES);
+      const int64_t slot = partial_slot<THREADS>(t0, at.t, at.tiles);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+#pragma unroll
+      for (int n0 = 0; n0 < NT; n0 += 2) {
+#pragma unroll
+        for (int n = n0; n < NT && n < n0 + 2; ++n)
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) buf[((n - n0) * 8 + t4 * 2 + i) * DP + ((k * 16 + e * 8 + g) ^ (t4 << 3))] = acc[n][k][e * 2 + i];
+        __syncwarp();
+#pragma unroll
+        for (int n = n0; n < NT && n < n0 + 2; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int r = n * 8 + c * 2 + i;
+              const float top = __shfl_sync(0xffffffffu, m[n][i], c), sum = __shfl_sync(0xffffffffu, l[n][i], c);
+              if (r >= nrows) continue;
+              const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key has no weight: zeros
+              const int64_t out = at.b * p.sob + row_head(p, hkv, row0 + r) * p.soh + row_token(p, row0 + r) * p.sos;
+              if (slot >= 0 && lane == 0) p.ml[slot * p.part_rows + r] = make_float2(top, sum);
+#pragma unroll
+              for (int d0 = 0; d0 < DP; d0 += 128) {
+                const int d = d0 + lane * 4;
+                if (d >= DP) break;
+                float4 v = *reinterpret_cast<const float4*>(buf + ((n - n0) * 8 + c * 2 + i) * DP + (d ^ (c << 3)));
+                if (slot < 0) {
+                  v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
+                  store_o4(p, out, d, v);
+                } else if (d < p.Dp) {
+                  *reinterpret_cast<float4*>(p.part + (slot * p.part_rows + r) * p.Dp + d) = v;
+                }
+              }
+            }
+        __syncwarp();
+      }
+      fresh = true;
+      if (left > 1) at.next_unit(p);
+    }
     fetch(stage);
     cp_async_commit();
     stage = stage + 1 == STAGES ? 0 : stage + 1;
-
-    if (++at.t < at.tiles && left > 1) continue;
-    // ---- the CTA leaves the unit: join the four warps, in turn so that the order is fixed
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
-        if (g == 0) {
-          wm[warp][n * 8 + t4 * 2 + i] = m[n][i];
-          wl[warp][n * 8 + t4 * 2 + i] = l[n][i];
-        }
-      }
-    __syncthreads();
-    for (int w = 0; w < 4; ++w) {
-      if (w == warp) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = n * 8 + t4 * 2 + i;
-            const float top = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-            const float scale = exp2_safe(m[n][i], top);
-#pragma unroll
-            for (int k = 0; k < KSTEPS; ++k)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float* o = obuf + r * OB + k * 16 + e * 8 + g;
-                *o = w == 0 ? acc[n][k][e * 2 + i] * scale : fmaf(acc[n][k][e * 2 + i], scale, *o);
-              }
-          }
-      }
-      __syncthreads();
-    }
-    const int64_t slot = partial_slot(t0, at.t, at.tiles);
-    for (int r = warp; r < nrows; r += 4) {
-      const int row = row0 + r;
-      const float top = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) sum = fmaf(wl[w][r], exp2_safe(wm[w][r], top), sum);
-      if (slot < 0) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key has no weight: zeros
-        const int64_t out = at.b * p.sob + row_head(p, hkv, row) * p.soh + row_token(p, row) * p.sos;
-        for (int d = lane; d < p.D; d += 32) store_from_f32(p.o, p.o_dtype, out + d, obuf[r * OB + d] * inv);
-      } else {
-        if (lane == 0) p.ml[slot * p.unit_rows + r] = make_float2(top, sum);
-        for (int d = lane; d < p.D; d += 32) p.part[(slot * p.unit_rows + r) * p.Dp + d] = obuf[r * OB + d];
-      }
-    }
-    __syncthreads();
-    fresh = true;
-    if (left > 1) at.next_unit(p);
   }
 }
-
-template <int DP>
-constexpr int n_tiles_max() { return DP == 256 ? 2 : 4; }
 
 // Query rows of a unit: eight, sixteen or thirty-two, whichever takes the rows of a kv head in
 // the fewest passes over its keys (32 x 256 accumulators would not fit the registers).
@@ -408,7 +379,7 @@ int n_tiles_for(int rows, int D) {
 typedef void (*PagedKernel)(const PagedParams);
 template <typename T, int DP, int NT>
 int launch(lh_ctx* ctx, const PagedParams& p, int ctas) {
-  constexpr int smem = 4 * Shape<DP>::stages * Shape<DP>::stage_bytes + NT * 8 * (DP + 4) * 4;
+  constexpr int smem = 4 * Shape<DP>::stages * Shape<DP>::stage_bytes;
   PagedKernel kernel = p.page % SUB == 0 ? paged_mma_kernel<T, DP, NT, true> : paged_mma_kernel<T, DP, NT, false>;
   LH_CUDA_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kernel<<<static_cast<unsigned>(ctas), THREADS, smem, ctx->stream>>>(p);
@@ -426,7 +397,9 @@ int launch_type(lh_ctx* ctx, const PagedParams& p, int ctas) {
 }  // namespace
 
 int paged_mma_unit_rows(int64_t rows, int D) { return 8 * n_tiles_for(rows > 64 ? 64 : static_cast<int>(rows), D); }
-int paged_mma_ctas(const lh_ctx* ctx, int D) { return ctx->sm_count * (D > 128 ? Shape<256>::ctas_per_sm : Shape<128>::ctas_per_sm); }
+int paged_mma_stretches(const lh_ctx* ctx, int D) {
+  return THREADS / 32 * ctx->sm_count * (D > 128 ? Shape<256>::ctas_per_sm : D > 64 ? Shape<128>::ctas_per_sm : Shape<64>::ctas_per_sm);
+}
 
 bool paged_mma_supported(const lh_memref_t* k, const lh_memref_t* v) {
   if ((k->dtype != LH_BF16 && k->dtype != LH_F16) || k->shape[3] % 8) return false;
@@ -438,8 +411,8 @@ bool paged_mma_supported(const lh_memref_t* k, const lh_memref_t* v) {
   return true;
 }
 
-int paged_mma_launch(lh_ctx* ctx, PagedParams& p, int dtype, int ctas) {
-  p.tile = TILE;
+int paged_mma_launch(lh_ctx* ctx, const PagedParams& p, int dtype, int stretches) {
+  const int ctas = stretches / (THREADS / 32);
   return dtype == LH_BF16 ? launch_type<__nv_bfloat16>(ctx, p, ctas) : launch_type<__half>(ctx, p, ctas);
 }
 
