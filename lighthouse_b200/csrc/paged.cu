@@ -461,12 +461,12 @@ struct JoinWork {
 
 __device__ __forceinline__ int64_t join_slot(const JoinWork& w, int c) { return c == 0 ? 2 * w.c0 + 1 : 2 * (w.c0 + c); }
 
-__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const PagedParams p, int64_t stretches) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32, 4) paged_join_kernel(const PagedParams p, int64_t stretches) {
   __shared__ JoinWork work[JOIN_WARPS];
   __shared__ float red[JOIN_WARPS];
   __shared__ float4 sums[JOIN_WARPS][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int ALONE = 8;  // parts that a warp adds up by itself
+  constexpr int ALONE = 32;  // parts that a warp adds up by itself
   grid_dependency_wait();
   if (blockIdx.y == 0) {
     const int64_t per = static_cast<int64_t>(p.Hkv) * p.group * p.Sq * p.D;
@@ -504,22 +504,21 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const Paged
       const float2 mine = lane < w.parts ? p.ml[join_slot(w, lane) * p.part_rows + r] : make_float2(-INFINITY, 0.f);
       float M = mine.x;
 #pragma unroll
-      for (int d = 4; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-      M = __shfl_sync(0xffffffffu, M, 0);
-      const float scale = exp2_safe(mine.x, M), weight = mine.y * scale;
-      float L = 0.f;
+      for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+      const float scale = exp2_safe(mine.x, M);
+      float L = mine.y * scale;
 #pragma unroll
-      for (int c = 0; c < ALONE; ++c) L += __shfl_sync(0xffffffffu, weight, c);
+      for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
       const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key has no weight: zeros
       const int row = row0 + r;
       const int64_t out = w.b * p.sob + row_head(p, hkv, row) * p.soh + row_token(p, row) * p.sos;
       for (int d0 = 0; d0 < p.Dp; d0 += 128) {
         const int d = d0 + lane * 4;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int c = 0; c < ALONE; ++c) {
+#pragma unroll 8
+        for (int c = 0; c < w.parts; ++c) {
           const float k = __shfl_sync(0xffffffffu, scale, c);
-          if (c < w.parts && d < p.Dp) {
+          if (d < p.Dp) {
             const float4 x = *reinterpret_cast<const float4*>(p.part + (join_slot(w, c) * p.part_rows + r) * p.Dp + d);
             a.x = fmaf(x.x, k, a.x); a.y = fmaf(x.y, k, a.y); a.z = fmaf(x.z, k, a.z); a.w = fmaf(x.w, k, a.w);
           }
@@ -766,7 +765,7 @@ extern "C" int lh_b200_paged_attention_workspace(lh_ctx_t* ctx, const lh_memref_
   const int Dp = static_cast<int>((q->shape[3] + 3) / 4 * 4), D = q->shape[3] > 256 ? 256 : static_cast<int>(q->shape[3]);
   const int64_t rows = q->shape[1] / k_pages->shape[2] * q->shape[2];
   const size_t simt = workspace_for(simt_stretches(ctx, D), std::min<int64_t>(rows, simt_unit_rows(rows)), Dp).bytes;
-  const size_t mma = workspace_for(paged_mma_stretches(ctx, D), std::min<int64_t>(rows, paged_mma_unit_rows(rows, D)), Dp).bytes;
+  const size_t mma = workspace_for(paged_mma_stretches(ctx, rows, D), std::min<int64_t>(rows, paged_mma_unit_rows(rows, D)), Dp).bytes;
   *bytes = std::max(simt, mma);
   return LH_OK;
 }
@@ -808,8 +807,9 @@ extern "C" int lh_b200_paged_attention(lh_ctx_t* ctx, const lh_memref_t* o, cons
   const bool mma = paged_mma_supported(k_pages, v_pages);
   p.unit_rows = mma ? paged_mma_unit_rows(p.rows, p.D) : simt_unit_rows(p.rows);
   p.part_rows = std::min(p.rows, p.unit_rows);
-  const int stretches = mma ? paged_mma_stretches(ctx, p.D) : simt_stretches(ctx, p.D);
+  const int stretches = mma ? paged_mma_stretches(ctx, p.rows, p.D) : simt_stretches(ctx, p.D);
   p.o_vec = p.D % 4 == 0 && aligned_view(o, 4);
+  p.q_pairs = dtype_size(q->dtype) == 2 && aligned_view(q, 2);
   p.row_groups = (p.rows + p.unit_rows - 1) / p.unit_rows;
   if (static_cast<int64_t>(p.Hkv) * p.row_groups > 0x7fffffffll) return set_error(ctx, LH_ERR_UNSUPPORTED, "paged_attention: too many query rows");
   const Workspace w = workspace_for(stretches, p.part_rows, p.Dp);

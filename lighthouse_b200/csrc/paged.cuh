@@ -28,6 +28,7 @@ struct PagedParams {
   int max_keys;           // table columns x page size
   int rows, unit_rows, row_groups;  // query rows of a kv head (tokens x group), rows of a unit, units of a kv head
   int o_dtype, o_vec;     // o_vec: four elements of a row of o can be stored at once
+  int q_pairs;            // two 16-bit elements of a row of q can be loaded at once
   float scale_log2;       // softmax scale x log2(e): scores are kept as powers of two
   // workspace
   int64_t* total;         // tiles of the whole call
@@ -42,7 +43,11 @@ constexpr int TILE = 16;  // keys of a tile
 constexpr int JOIN_WARPS = 8;
 
 // Stretch i of n is tiles [total * i / n, total * (i + 1) / n); none is empty because n <= total.
-__host__ __device__ __forceinline__ int64_t stretch_begin(int64_t total, int64_t n, int64_t i) { return total * i / n; }
+// (n is some thousands at most, so 32-bit division serves all but the longest calls in a quarter of the time.)
+__host__ __device__ __forceinline__ int64_t stretch_begin(int64_t total, int64_t n, int64_t i) {
+  const int64_t x = total * i;
+  return x < 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(n)) : x / n;
+}
 // The stretch that has tile x: the last i with total * i / n < x + 1.
 __host__ __device__ __forceinline__ int64_t stretch_owner(int64_t total, int64_t n, int64_t x) { return ((x + 1) * n - 1) / total; }
 
@@ -61,8 +66,9 @@ struct TileCursor {
     b = b_;
     len = paged_length(p, b);
     tiles = paged_tiles(len);
-    u = static_cast<int>(within / tiles);
-    t = static_cast<int>(within % tiles);
+    // a sequence has at most 2^27 tiles, and its units are as many as fit 31 bits: only the longest need 64
+    u = within < 0x7fffffff ? static_cast<int>(static_cast<uint32_t>(within) / static_cast<uint32_t>(tiles)) : static_cast<int>(within / tiles);
+    t = static_cast<int>(within - static_cast<int64_t>(u) * tiles);
   }
   // Only called while tiles of this warp's stretch remain, so the next sequence exists.
   __device__ __forceinline__ void next_unit(const PagedParams& p) {
@@ -208,7 +214,7 @@ __device__ __forceinline__ int row_head(const PagedParams& p, int hkv, int row) 
 // The tensor-core kernel (paged_mma.cu).
 bool paged_mma_supported(const lh_memref_t* k, const lh_memref_t* v);
 int paged_mma_unit_rows(int64_t rows, int D);
-int paged_mma_stretches(const lh_ctx* ctx, int D);
+int paged_mma_stretches(const lh_ctx* ctx, int64_t rows, int D);
 int paged_mma_launch(lh_ctx* ctx, const PagedParams& p, int dtype, int stretches);
 
 }  // namespace lh

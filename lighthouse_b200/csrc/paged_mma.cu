@@ -26,11 +26,14 @@ namespace {
 constexpr int THREADS = 128;
 constexpr int SUB = TILE;
 
-template <int DP>
+// Stages of a warp's ring and CTAs of an SM. A tile takes a warp about 1500 clocks from ldmatrix to the
+// next fetch, most of them latency, and its loads are there before it asks for them: more warps
+// are worth more than deeper rings, as far as the accumulators leave registers for them.
+template <int DP, int NT>
 struct Shape {
   static constexpr int stage_bytes = 2 * SUB * DP * 2;  // K and V rows of 16 keys
-  static constexpr int stages = DP == 64 ? 6 : 3;
-  static constexpr int ctas_per_sm = DP == 256 ? 1 : 2;
+  static constexpr int ctas_per_sm = DP == 256 ? 1 : NT == 1 ? 3 : 2;
+  static constexpr int stages = DP == 64 ? (NT == 1 ? 4 : 6) : DP == 128 ? (NT == 1 ? 2 : 3) : 3;
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -74,15 +77,116 @@ __device__ __forceinline__ float bits_to_f32(uint32_t bits16) {
   else return __uint_as_float(bits16 << 16);
 }
 
+// The side of a warp that fetches. It knows the next tile and looks pages up ahead of their use: where a
+// tile lies within one page (WHOLE_PAGE) those of 32 tiles at once, one per lane; else those of the
+// next tile's 16 keys.
+template <typename T, int DP, bool WHOLE_PAGE>
+struct Producer {
+  static constexpr int CHUNKS = DP / 8;             // 16-byte chunks of a row
+  static constexpr int ROWS_AT_ONCE = 32 / CHUNKS;  // rows that one cp.async per lane covers
+  TileCursor at;
+  int64_t left;  // tiles still to fetch
+  int page_id, first;  // looked up; the tile that lane 0's page is of
+  int64_t k_head, v_head;
+
+  __device__ __forceinline__ void begin(const PagedParams& p, const TileCursor& from, int64_t n) {
+    at = from;
+    left = n;
+    enter_unit(p);
+  }
+  __device__ __forceinline__ void enter_unit(const PagedParams& p) {
+    const int hkv = at.u / p.row_groups;
+    k_head = hkv * p.skh;
+    v_head = hkv * p.svh;
+    look_up(p);
+  }
+  __device__ __forceinline__ void look_up(const PagedParams& p) {
+    const int lane = threadIdx.x & 31;
+    first = at.t;
+    const int64_t j = WHOLE_PAGE ? (static_cast<int64_t>(at.t) + lane) * TILE : at.t * TILE + (lane & 15);
+    page_id = j < at.len ? p.table[at.b * p.stb + page_of(p, static_cast<int>(j)) * p.stp] : -1;
+  }
+  // Starts the copies of the next tile into a stage; returns which of its keys exist.
+  __device__ __forceinline__ uint32_t fetch(const PagedParams& p, const T* K, const T* V, uint32_t stage) {
+    const int lane = threadIdx.x & 31, chunk = lane % CHUNKS, row_in = lane / CHUNKS;
+    const bool chunk_there = chunk * 8 < p.D;
+    const int key0 = at.t * TILE;
+    constexpr uint32_t V_OFF = SUB * DP * 2;
+    // (row & 7) of rows ROWS_AT_ONCE apart: the swizzle's pattern repeats over the rows
+    uint32_t mask;
+    if constexpr (WHOLE_PAGE) {
+      const int id = __shfl_sync(0xffffffffu, page_id, at.t - first);
+      const int n = at.len - key0;
+      const bool inside = id >= 0 && id < p.num_pages;
+      mask = !inside ? 0u : n >= SUB ? 0xffffu : (1u << n) - 1u;
+      if (!inside && lane == 0) report_bad_index(p.dev_status);
+      if (mask) {
+        const int slot = key0 - page_of(p, key0) * p.page;
+        const T* ks = K + id * p.skp + (slot + row_in) * p.sks + k_head + chunk * 8;
+        const T* vs = V + id * p.svp + (slot + row_in) * p.svs + v_head + chunk * 8;
+        if (mask == 0xffffu && DP == p.D) {
+#pragma unroll
+          for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
+            const int row = i * ROWS_AT_ONCE + row_in;
+            const uint32_t dst = stage + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
+            cp_async16(dst, ks, 16);
+            cp_async16(dst + V_OFF, vs, 16);
+            ks += ROWS_AT_ONCE * p.sks;
+            vs += ROWS_AT_ONCE * p.svs;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
+            const int row = i * ROWS_AT_ONCE + row_in;
+            const bool get = chunk_there && (mask >> row & 1);
+            const uint32_t dst = stage + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
+            cp_async16(dst, get ? ks : K, get ? 16 : 0);
+            cp_async16(dst + V_OFF, get ? vs : V, get ? 16 : 0);
+            ks += ROWS_AT_ONCE * p.sks;
+            vs += ROWS_AT_ONCE * p.svs;
+          }
+        }
+      }
+    } else {
+      const int j = key0 + (lane & 15);
+      const bool live = j < at.len, inside = page_id >= 0 && page_id < p.num_pages;
+      if (live && !inside) report_bad_index(p.dev_status);
+      mask = __ballot_sync(0xffffffffu, live && inside) & 0xffffu;
+      const int slot = j - page_of(p, j) * p.page;
+      const int64_t ko = live && inside ? page_id * p.skp + slot * p.sks + k_head : 0;
+      const int64_t vo = live && inside ? page_id * p.svp + slot * p.svs + v_head : 0;
+      if (mask) {
+#pragma unroll
+        for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
+          const int row = i * ROWS_AT_ONCE + row_in;
+          const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
+          const bool get = chunk_there && (mask >> row & 1);
+          const uint32_t dst = stage + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
+          cp_async16(dst, get ? K + kr + chunk * 8 : K, get ? 16 : 0);
+          cp_async16(dst + V_OFF, get ? V + vr + chunk * 8 : V, get ? 16 : 0);
+        }
+      }
+    }
+    --left;
+    if (++at.t == at.tiles) {
+      if (left > 0) {
+        at.next_unit(p);
+        enter_unit(p);
+      }
+    } else if (!WHOLE_PAGE || at.t - first == 32) {
+      look_up(p);
+    }
+    return mask;
+  }
+};
+
 template <typename T, int DP, int NT, bool WHOLE_PAGE>
-__global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_kernel(const PagedParams p) {
-  constexpr int STAGES = Shape<DP>::stages, STAGE_BYTES = Shape<DP>::stage_bytes, V_OFF = STAGE_BYTES / 2;
-  constexpr int CHUNKS = DP / 8;             // 16-byte chunks of a row
-  constexpr int ROWS_AT_ONCE = 32 / CHUNKS;  // rows that one cp.async per lane covers
+__global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma_kernel(const PagedParams p) {
+  constexpr int STAGES = Shape<DP, NT>::stages, STAGE_BYTES = Shape<DP, NT>::stage_bytes, V_OFF = STAGE_BYTES / 2;
   constexpr int KSTEPS = DP / 16;
   extern __shared__ __align__(128) char smem[];
   __shared__ uint32_t there[4][STAGES];  // which of a stage's 16 keys exist
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   grid_dependency_trigger();
   int64_t lo, hi;
@@ -93,129 +197,93 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
   char* const ring_ptr = smem + warp * STAGES * STAGE_BYTES;
   const T* const K = static_cast<const T*>(p.k);
   const T* const V = static_cast<const T*>(p.v);
-
-  // ---- producer
-  const int chunk = lane % CHUNKS, row_in = lane / CHUNKS;
-  const bool chunk_there = chunk * 8 < p.D;
-  Fetch f;
-  f.at = at;
-  f.left = hi - lo;
-  const int my_key = WHOLE_PAGE ? 0 : lane & 15;  // WHOLE_PAGE: a tile lies within one page
-  f.look_up(p, my_key);
+  Producer<T, DP, WHOLE_PAGE> producer;
+  producer.begin(p, at, hi - lo);
   auto fetch = [&](int stage) {
-    if (f.left <= 0) return;
-    const int key0 = f.at.t * TILE;
-    const int hkv = f.at.u / p.row_groups;
-    const bool inside = f.page_id >= 0 && f.page_id < p.num_pages;
-    const uint32_t base = ring + stage * STAGE_BYTES;
-    uint32_t mask;
-    if constexpr (WHOLE_PAGE) {
-      const int n = f.at.len - key0;
-      mask = !inside ? 0u : n >= SUB ? 0xffffu : (1u << n) - 1u;
-      if (n > 0 && !inside && lane == 0) report_bad_index(p.dev_status);
-      if (mask) {
-        const int slot = key0 - page_of(p, key0) * p.page;
-        const T* ks = K + f.page_id * p.skp + slot * p.sks + hkv * p.skh + chunk * 8;
-        const T* vs = V + f.page_id * p.svp + slot * p.svs + hkv * p.svh + chunk * 8;
-#pragma unroll
-        for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
-          const int row = i * ROWS_AT_ONCE + row_in;
-          const bool get = chunk_there && (mask >> row & 1);
-          const uint32_t dst = base + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
-          cp_async16(dst, get ? ks + row * p.sks : K, get ? 16 : 0);
-          cp_async16(dst + V_OFF, get ? vs + row * p.svs : V, get ? 16 : 0);
-        }
-      }
-    } else {
-      const int j = key0 + (lane & 15);
-      const bool live = j < f.at.len;
-      if (live && !inside) report_bad_index(p.dev_status);
-      mask = __ballot_sync(0xffffffffu, live && inside) & 0xffffu;
-      const int slot = j - page_of(p, j) * p.page;
-      const int64_t ko = live && inside ? f.page_id * p.skp + slot * p.sks + hkv * p.skh : 0;
-      const int64_t vo = live && inside ? f.page_id * p.svp + slot * p.svs + hkv * p.svh : 0;
-      if (mask) {
-#pragma unroll
-        for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
-          const int row = i * ROWS_AT_ONCE + row_in;
-          const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
-          const bool get = chunk_there && (mask >> row & 1);
-          const uint32_t dst = base + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
-          cp_async16(dst, get ? K + kr + chunk * 8 : K, get ? 16 : 0);
-          cp_async16(dst + V_OFF, get ? V + vr + chunk * 8 : V, get ? 16 : 0);
-        }
-      }
+    if (producer.left > 0) {
+      const uint32_t mask = producer.fetch(p, K, V, ring + stage * STAGE_BYTES);
+      if (lane == 0) there[warp][stage] = mask;
     }
-    if (lane == 0) there[warp][stage] = mask;
-    f.advance(p);
-    f.look_up(p, my_key);
-  };
-#pragma unroll
-  for (int s = 0; s < STAGES; ++s) {
-    fetch(s);
     cp_async_commit();
-  }
+  };
 
-  // ---- consumer
-  // ldmatrix addresses inside a stage: lane l gives row (l & 7) of matrix l / 8
-  const int mi = lane >> 3, r8 = lane & 7;
-  const int krow = (mi & 1) * 8 + r8, kchunk = mi >> 1;  // K: matrices (keys lo, k lo), (keys hi, k lo), (keys lo, k hi), (keys hi, k hi)
-  const int vrow = (mi >> 1) * 8 + r8, vchunk = mi & 1;  // V, transposed: (dims lo, keys lo), (dims hi, keys lo), (dims lo, keys hi), (dims hi, keys hi)
+  // ---- a unit: lane r knows query row r of it, the fragments of Q are loaded
   uint32_t qf[NT][KSTEPS][2];
-  float acc[NT][KSTEPS][4];
-  float m[NT][2], l[NT][2];  // query rows 2 t4 and 2 t4 + 1 of each n tile
-  int seen[NT][2];
-  int t0 = at.t, stage = 0;
-  bool fresh = true;
-  for (int64_t left = hi - lo; left > 0; --left) {
-    const int hkv = at.u / p.row_groups, row0 = (at.u % p.row_groups) * (NT * 8);
-    const int nrows = min(NT * 8, p.rows - row0);
-    if (fresh) {
-      fresh = false;
-      t0 = at.t;
+  int64_t o_row;          // lane r: offset of row r of o
+  int nrows, seen[NT][2]; // rows; keys that rows 2 t4 and 2 t4 + 1 of each n tile may see
+  int t0;
+  auto enter_unit = [&]() {
+    const int hkv = at.u / p.row_groups, row0 = (at.u - hkv * p.row_groups) * (NT * 8);
+    nrows = min(NT * 8, p.rows - row0);
+    t0 = at.t;
+    const int token = (row0 + lane) / p.group, head = hkv * p.group + (row0 + lane) - token * p.group;
+    o_row = at.b * p.sob + head * p.soh + token * p.sos;
+    const int64_t q_row = at.b * p.sqb + head * p.sqh + token * p.sqs;
+    const int sees = at.len - p.Sq + 1 + token;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int r = n * 8 + g, row = row0 + r;
-        const T* q = static_cast<const T*>(p.q) + at.b * p.sqb + (r < nrows ? row_head(p, hkv, row) * p.sqh + row_token(p, row) * p.sqs : 0);
+    for (int n = 0; n < NT; ++n) {
+      seen[n][0] = __shfl_sync(0xffffffffu, sees, n * 8 + t4 * 2);
+      seen[n][1] = __shfl_sync(0xffffffffu, sees, n * 8 + t4 * 2 + 1);
+      const bool is = n * 8 + g < nrows;
+      const int64_t off = __shfl_sync(0xffffffffu, q_row, n * 8 + g);
+      const unsigned short* const q = static_cast<const unsigned short*>(p.q) + (is ? off : 0) + t4 * 2;
+      if (p.q_pairs) {
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) qf[n][k][i] = is && k * 16 + i * 8 + t4 * 2 < p.D ? *reinterpret_cast<const uint32_t*>(q + k * 16 + i * 8) : 0u;
+      } else {
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int d = k * 16 + i * 8 + t4 * 2;
-            const unsigned short* q16 = reinterpret_cast<const unsigned short*>(q) + d;
-            const uint32_t a = r < nrows && d < p.D ? q16[0] : 0u, b = r < nrows && d + 1 < p.D ? q16[1] : 0u;
-            qf[n][k][i] = a | b << 16;
+            const bool in = is && k * 16 + i * 8 + t4 * 2 < p.D;  // D is a multiple of eight
+            qf[n][k][i] = in ? q[k * 16 + i * 8] | static_cast<uint32_t>(q[k * 16 + i * 8 + 1]) << 16 : 0u;
           }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          m[n][i] = -INFINITY;
-          l[n][i] = 0.f;
-          const int mine = row0 + n * 8 + t4 * 2 + i;
-          seen[n][i] = at.len - p.Sq + 1 + row_token(p, mine);
-        }
-#pragma unroll
-        for (int k = 0; k < KSTEPS; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[n][k][i] = 0.f;
       }
     }
+  };
+  enter_unit();
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) fetch(s);
+
+  // ldmatrix addresses inside a stage: lane l gives row (l & 7) of matrix l / 8
+  const int mi = lane >> 3, r8 = lane & 7;
+  const int krow = (mi & 1) * 8 + r8, kchunk = mi >> 1;  // K: matrices (keys lo, k lo), (keys hi, k lo), (keys lo, k hi), (keys hi, k hi)
+  const int vrow = (mi >> 1) * 8 + r8, vchunk = mi & 1;  // V, transposed: (dims lo, keys lo), (dims hi, keys lo), (dims lo, keys hi), (dims hi, keys hi)
+  float acc[NT][KSTEPS][4];
+  float m[NT][2], l[NT][2];  // query rows 2 t4 and 2 t4 + 1 of each n tile
+  auto clear = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][k][i] = 0.f;
+    }
+  };
+  clear();
+  int stage = 0;
+  for (int64_t left = hi - lo; left > 0; --left) {
     cp_async_wait<STAGES - 1>();
     __syncwarp();
     const uint32_t mask = there[warp][stage];
     if (mask) {
       const uint32_t base = ring + stage * STAGE_BYTES;
       const int key0 = at.t * TILE;
-      float s[NT][4];
+      float s[NT][4], s2[NT][4];  // even and odd steps: two chains of half the length
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+        for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
         uint32_t a[4];
         ldmatrix4(a, base + krow * (DP * 2) + (((k * 2 + kchunk) ^ (krow & 7)) << 4));
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<T>(s[n], a, qf[n][k][0], qf[n][k][1]);
+        for (int n = 0; n < NT; ++n) mma16816<T>(k & 1 ? s2[n] : s[n], a, qf[n][k][0], qf[n][k][1]);
       }
       const bool some_masked = key0 + SUB > at.len - p.Sq + 1;  // some row does not see some of these keys (or they do not exist)
       const bool whole = mask == 0xffffu && !some_masked;
@@ -224,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[n][i] *= p.scale_log2;
+          s[n][i] = (s[n][i] + s2[n][i]) * p.scale_log2;
           if (!whole) {
             const int key = g + (i >> 1) * 8;
             if (!(mask >> key & 1) || key0 + key >= seen[n][i & 1]) s[n][i] = -INFINITY;
@@ -313,58 +381,62 @@ __global__ void __launch_bounds__(THREADS, Shape<DP>::ctas_per_sm) paged_mma_ker
     __syncwarp();
     if (++at.t == at.tiles || left == 1) {
       // ---- the warp leaves the unit. The stage just used takes two n tiles of results as rows of f32;
-      // dimensions are swizzled by the row so that neither side meets in a bank.
+      // dimensions are swizzled by the row so that neither side meets in a bank. The next unit's
+      // Q is on its way meanwhile.
       float* const buf = reinterpret_cast<float*>(ring_ptr + stage * STAGE_BYTES);
       const int64_t slot = partial_slot<THREADS>(t0, at.t, at.tiles);
+      const int64_t rows_at = slot < 0 ? o_row : (slot * p.part_rows + lane) * p.Dp;
+      const int n_done = nrows;
+      if (left > 1) {
+        at.next_unit(p);
+        enter_unit();
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+      if (slot >= 0 && g == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (n * 8 + t4 * 2 + i < n_done) p.ml[slot * p.part_rows + n * 8 + t4 * 2 + i] = make_float2(m[n][i], l[n][i]);
+      }
 #pragma unroll
       for (int n0 = 0; n0 < NT; n0 += 2) {
 #pragma unroll
         for (int n = n0; n < NT && n < n0 + 2; ++n)
 #pragma unroll
-          for (int k = 0; k < KSTEPS; ++k)
+          for (int i = 0; i < 2; ++i) {
+            // a row that sees no key has no weight: zeros
+            const float inv = slot >= 0 ? 1.f : l[n][i] == 0.f ? 0.f : 1.f / l[n][i];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) buf[((n - n0) * 8 + t4 * 2 + i) * DP + ((k * 16 + e * 8 + g) ^ (t4 << 3))] = acc[n][k][e * 2 + i];
+              for (int e = 0; e < 2; ++e) buf[((n - n0) * 8 + t4 * 2 + i) * DP + ((k * 16 + e * 8 + g) ^ (t4 << 3))] = acc[n][k][e * 2 + i] * inv;
+          }
         __syncwarp();
+#pragma unroll 4
+        for (int q = 0; q < 16; ++q) {
+          const int r = n0 * 8 + q;
+          if (r >= n_done || (NT == 1 && q >= 8)) break;
+          const int64_t to = __shfl_sync(0xffffffffu, rows_at, r);
 #pragma unroll
-        for (int n = n0; n < NT && n < n0 + 2; ++n)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int r = n * 8 + c * 2 + i;
-              const float top = __shfl_sync(0xffffffffu, m[n][i], c), sum = __shfl_sync(0xffffffffu, l[n][i], c);
-              if (r >= nrows) continue;
-              const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key has no weight: zeros
-              const int64_t out = at.b * p.sob + row_head(p, hkv, row0 + r) * p.soh + row_token(p, row0 + r) * p.sos;
-              if (slot >= 0 && lane == 0) p.ml[slot * p.part_rows + r] = make_float2(top, sum);
-#pragma unroll
-              for (int d0 = 0; d0 < DP; d0 += 128) {
-                const int d = d0 + lane * 4;
-                if (d >= DP) break;
-                float4 v = *reinterpret_cast<const float4*>(buf + ((n - n0) * 8 + c * 2 + i) * DP + (d ^ (c << 3)));
-                if (slot < 0) {
-                  v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-                  store_o4(p, out, d, v);
-                } else if (d < p.Dp) {
-                  *reinterpret_cast<float4*>(p.part + (slot * p.part_rows + r) * p.Dp + d) = v;
-                }
-              }
-            }
+          for (int d0 = 0; d0 < DP; d0 += 128) {
+            const int d = d0 + lane * 4;
+            if (d >= DP) break;
+            const float4 v = *reinterpret_cast<const float4*>(buf + q * DP + (d ^ ((q >> 1 & 3) << 3)));
+            if (slot < 0) store_o4(p, to, d, v);
+            else if (d < p.Dp) *reinterpret_cast<float4*>(p.part + to + d) = v;
+          }
+        }
         __syncwarp();
       }
-      fresh = true;
-      if (left > 1) at.next_unit(p);
+      clear();
     }
     fetch(stage);
-    cp_async_commit();
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
 }
@@ -379,7 +451,7 @@ int n_tiles_for(int rows, int D) {
 typedef void (*PagedKernel)(const PagedParams);
 template <typename T, int DP, int NT>
 int launch(lh_ctx* ctx, const PagedParams& p, int ctas) {
-  constexpr int smem = 4 * Shape<DP>::stages * Shape<DP>::stage_bytes;
+  constexpr int smem = THREADS / 32 * Shape<DP, NT>::stages * Shape<DP, NT>::stage_bytes;
   PagedKernel kernel = p.page % SUB == 0 ? paged_mma_kernel<T, DP, NT, true> : paged_mma_kernel<T, DP, NT, false>;
   LH_CUDA_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kernel<<<static_cast<unsigned>(ctas), THREADS, smem, ctx->stream>>>(p);
@@ -397,8 +469,11 @@ int launch_type(lh_ctx* ctx, const PagedParams& p, int ctas) {
 }  // namespace
 
 int paged_mma_unit_rows(int64_t rows, int D) { return 8 * n_tiles_for(rows > 64 ? 64 : static_cast<int>(rows), D); }
-int paged_mma_stretches(const lh_ctx* ctx, int D) {
-  return THREADS / 32 * ctx->sm_count * (D > 128 ? Shape<256>::ctas_per_sm : D > 64 ? Shape<128>::ctas_per_sm : Shape<64>::ctas_per_sm);
+int paged_mma_stretches(const lh_ctx* ctx, int64_t rows, int D) {
+  const bool one = paged_mma_unit_rows(rows, D) == 8;
+  const int ctas = D > 128 ? Shape<256, 1>::ctas_per_sm : one ? Shape<128, 1>::ctas_per_sm : Shape<128, 2>::ctas_per_sm;
+  static_assert(Shape<64, 1>::ctas_per_sm == Shape<128, 1>::ctas_per_sm && Shape<64, 2>::ctas_per_sm == Shape<128, 2>::ctas_per_sm && Shape<256, 1>::ctas_per_sm == Shape<256, 2>::ctas_per_sm && Shape<128, 2>::ctas_per_sm == Shape<128, 4>::ctas_per_sm, "one rule for all");
+  return THREADS / 32 * ctx->sm_count * ctas;
 }
 
 bool paged_mma_supported(const lh_memref_t* k, const lh_memref_t* v) {
