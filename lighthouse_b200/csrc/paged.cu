@@ -482,13 +482,13 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) paged_join_kernel(const Pa
   const int64_t i = static_cast<int64_t>(blockIdx.x) * JOIN_WARPS + warp;
   JoinWork w = {0, 0, 0, 0};
   if (i > 0 && i < stretches) {
-    const int4 here = p.first[i];
+    const int4 here = p.first[i];  // the unit's tiles with it: nothing to look up in turn
     if (here.x >= 0 && here.z > 0) {  // a stretch that begins inside its unit
       const int64_t total = *p.total;
       const int64_t n = total < stretches ? total : stretches;
       const int64_t begin = stretch_begin(total, n, i) - here.z;
       if (stretch_begin(total, n, i - 1) <= begin) {  // no earlier border lies in this unit
-        const int64_t end = begin + paged_tiles(paged_length(p, here.x));
+        const int64_t end = begin + here.w;
         w.c0 = i - 1;
         w.parts = static_cast<int>(stretch_owner(total, n, end - 1) - w.c0 + 1);
         w.b = here.x;
@@ -515,12 +515,21 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) paged_join_kernel(const Pa
       for (int d0 = 0; d0 < p.Dp; d0 += 128) {
         const int d = d0 + lane * 4;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int c = 0; c < w.parts; ++c) {
-          const float k = __shfl_sync(0xffffffffu, scale, c);
-          if (d < p.Dp) {
-            const float4 x = *reinterpret_cast<const float4*>(p.part + (join_slot(w, c) * p.part_rows + r) * p.Dp + d);
-            a.x = fmaf(x.x, k, a.x); a.y = fmaf(x.y, k, a.y); a.z = fmaf(x.z, k, a.z); a.w = fmaf(x.w, k, a.w);
+        // parts lie two slots apart, but for the first; six of them are on their way at a time
+        const int64_t apart = 2 * static_cast<int64_t>(p.part_rows) * p.Dp;
+        const float* const first = p.part + (join_slot(w, 0) * p.part_rows + r) * p.Dp + (d < p.Dp ? d : 0);
+        const float* const rest = first - apart / 2;
+        constexpr int BATCH = 6;
+        for (int c0 = 0; c0 < w.parts; c0 += BATCH) {
+          float4 x[BATCH];
+#pragma unroll
+          for (int c = 0; c < BATCH; ++c) x[c] = *reinterpret_cast<const float4*>(c0 + c == 0 ? first : rest + min(c0 + c, w.parts - 1) * apart);
+#pragma unroll
+          for (int c = 0; c < BATCH; ++c) {
+            const float k = __shfl_sync(0xffffffffu, scale, min(c0 + c, 31));
+            if (c0 + c < w.parts) {
+              a.x = fmaf(x[c].x, k, a.x); a.y = fmaf(x[c].y, k, a.y); a.z = fmaf(x[c].z, k, a.z); a.w = fmaf(x[c].w, k, a.w);
+            }
           }
         }
         store_o4(p, out, d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));

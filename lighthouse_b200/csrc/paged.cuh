@@ -32,7 +32,7 @@ struct PagedParams {
   float scale_log2;       // softmax scale x log2(e): scores are kept as powers of two
   // workspace
   int64_t* total;         // tiles of the whole call
-  int4* first;            // per stretch: (sequence, unit, tile) it starts at; x < 0: it has none
+  int4* first;            // per stretch: (sequence, unit, tile) it starts at and the unit's tiles; x < 0: it has none
   float2* ml;             // per partial row: running maximum and sum
   float* part;            // per partial row: Dp floats, not yet divided by the sum
   int Dp, part_rows;      // floats of a partial row, rows of a partial result
@@ -146,7 +146,7 @@ __device__ __forceinline__ bool find_stretch(const PagedParams& p, int64_t& lo, 
   lo = stretch_begin(total, n, s);
   hi = stretch_begin(total, n, s + 1);
   at.seek(p, start_b[warp], lo - start_base[warp]);
-  if (lane == 0) p.first[s] = make_int4(at.b, at.u, at.t, 0);
+  if (lane == 0) p.first[s] = make_int4(at.b, at.u, at.t, at.tiles);
   return true;
 }
 

@@ -12,10 +12,13 @@
 // first product with keys along the rows; movmatrix turns its 8 x 8 blocks into the second
 // product's operand in registers.
 //
-// Each warp runs by itself, on its own stretch of tiles: it fetches 16 keys at a time with cp.async
-// into a ring of its own and keeps its own online softmax, so nothing in the kernel after its
-// first microsecond waits for another warp. At the end of a unit the results are turned to rows in
-// the stage just used, while the ring is already being filled for the next unit.
+// Each warp runs by itself, on its own stretch of tiles: its first lane has the TMA bring 16 keys at a
+// time into a ring of the warp's own (one box per 64 dimensions, 128-byte swizzle), and the warp keeps
+// its own online softmax, so nothing in the kernel after its first microsecond waits for another
+// warp. (With cp.async in its place the addresses of 32 copies per lane and tile were half of all
+// instructions, and the kernel was bound by their issue.) Tiles that lie across pages, and pools
+// that no tensor map describes, are fetched with cp.async, row by row. At the end of a unit the
+// results are turned to rows in the stage just used, while the ring is being filled for the next.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -77,17 +80,19 @@ __device__ __forceinline__ float bits_to_f32(uint32_t bits16) {
   else return __uint_as_float(bits16 << 16);
 }
 
-// The side of a warp that fetches. It knows the next tile and looks pages up ahead of their use: where a
-// tile lies within one page (WHOLE_PAGE) those of 32 tiles at once, one per lane; else those of the
-// next tile's 16 keys.
-template <typename T, int DP, bool WHOLE_PAGE>
+// Where 16-byte chunk `chunk` of row `row` of K or V lies in its half of a stage: blocks of 16 rows x 64
+// dimensions, chunks swizzled by the row, as the TMA writes them.
+__device__ __forceinline__ uint32_t place_of(int row, int chunk) { return (chunk >> 3) * (SUB * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
+
+// The side of a warp that fetches. It knows the next tile and looks pages up ahead of their use: with
+// the TMA, where a tile lies within one page, those of 32 tiles at once, one per lane; else those
+// of the next tile's 16 keys.
+template <typename T, int DP, bool TMA>
 struct Producer {
-  static constexpr int CHUNKS = DP / 8;             // 16-byte chunks of a row
-  static constexpr int ROWS_AT_ONCE = 32 / CHUNKS;  // rows that one cp.async per lane covers
   TileCursor at;
   int64_t left;  // tiles still to fetch
   int page_id, first;  // looked up; the tile that lane 0's page is of
-  int64_t k_head, v_head;
+  int hkv;
 
   __device__ __forceinline__ void begin(const PagedParams& p, const TileCursor& from, int64_t n) {
     at = from;
@@ -95,73 +100,62 @@ struct Producer {
     enter_unit(p);
   }
   __device__ __forceinline__ void enter_unit(const PagedParams& p) {
-    const int hkv = at.u / p.row_groups;
-    k_head = hkv * p.skh;
-    v_head = hkv * p.svh;
+    hkv = at.u / p.row_groups;
     look_up(p);
   }
   __device__ __forceinline__ void look_up(const PagedParams& p) {
     const int lane = threadIdx.x & 31;
     first = at.t;
-    const int64_t j = WHOLE_PAGE ? (static_cast<int64_t>(at.t) + lane) * TILE : at.t * TILE + (lane & 15);
+    const int64_t j = TMA ? (static_cast<int64_t>(at.t) + lane) * TILE : at.t * TILE + (lane & 15);
     page_id = j < at.len ? p.table[at.b * p.stb + page_of(p, static_cast<int>(j)) * p.stp] : -1;
   }
-  // Starts the copies of the next tile into a stage; returns which of its keys exist.
-  __device__ __forceinline__ uint32_t fetch(const PagedParams& p, const T* K, const T* V, uint32_t stage) {
-    const int lane = threadIdx.x & 31, chunk = lane % CHUNKS, row_in = lane / CHUNKS;
-    const bool chunk_there = chunk * 8 < p.D;
+  // Starts the copies of the next tile into a stage; returns which of its keys exist. With the TMA they
+  // complete on `full`, without on the warp's cp.async group.
+  __device__ __forceinline__ uint32_t fetch(const PagedParams& p, const CUtensorMap* tm_k, const CUtensorMap* tm_v, char* stage, uint64_t* full) {
+    const int lane = threadIdx.x & 31;
     const int key0 = at.t * TILE;
-    constexpr uint32_t V_OFF = SUB * DP * 2;
-    // (row & 7) of rows ROWS_AT_ONCE apart: the swizzle's pattern repeats over the rows
+    constexpr int V_OFF = SUB * DP * 2;
     uint32_t mask;
-    if constexpr (WHOLE_PAGE) {
+    if constexpr (TMA) {
       const int id = __shfl_sync(0xffffffffu, page_id, at.t - first);
       const int n = at.len - key0;
       const bool inside = id >= 0 && id < p.num_pages;
       mask = !inside ? 0u : n >= SUB ? 0xffffu : (1u << n) - 1u;
-      if (!inside && lane == 0) report_bad_index(p.dev_status);
-      if (mask) {
-        const int slot = key0 - page_of(p, key0) * p.page;
-        const T* ks = K + id * p.skp + (slot + row_in) * p.sks + k_head + chunk * 8;
-        const T* vs = V + id * p.svp + (slot + row_in) * p.svs + v_head + chunk * 8;
-        if (mask == 0xffffu && DP == p.D) {
+      if (lane == 0) {
+        if (inside) {
+          const int slot = key0 - page_of(p, key0) * p.page;
+          mbar_arrive_expect_tx(full, 2 * V_OFF);
 #pragma unroll
-          for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
-            const int row = i * ROWS_AT_ONCE + row_in;
-            const uint32_t dst = stage + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
-            cp_async16(dst, ks, 16);
-            cp_async16(dst + V_OFF, vs, 16);
-            ks += ROWS_AT_ONCE * p.sks;
-            vs += ROWS_AT_ONCE * p.svs;
+          for (int c = 0; c < DP / 64; ++c) {
+            tma_load_4d(stage + c * (SUB * 128), tm_k, full, c * 64, slot, hkv, id);
+            tma_load_4d(stage + V_OFF + c * (SUB * 128), tm_v, full, c * 64, slot, hkv, id);
           }
         } else {
-#pragma unroll
-          for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
-            const int row = i * ROWS_AT_ONCE + row_in;
-            const bool get = chunk_there && (mask >> row & 1);
-            const uint32_t dst = stage + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
-            cp_async16(dst, get ? ks : K, get ? 16 : 0);
-            cp_async16(dst + V_OFF, get ? vs : V, get ? 16 : 0);
-            ks += ROWS_AT_ONCE * p.sks;
-            vs += ROWS_AT_ONCE * p.svs;
-          }
+          report_bad_index(p.dev_status);
         }
       }
     } else {
+      constexpr int CHUNKS = DP / 8;             // 16-byte chunks of a row
+      constexpr int ROWS_AT_ONCE = 32 / CHUNKS;  // rows that one cp.async per lane covers
+      const T* const K = static_cast<const T*>(p.k);
+      const T* const V = static_cast<const T*>(p.v);
+      const uint32_t to = smem_u32(stage);
+      const int chunk = lane % CHUNKS, row_in = lane / CHUNKS;
+      const bool chunk_there = chunk * 8 < p.D;
       const int j = key0 + (lane & 15);
       const bool live = j < at.len, inside = page_id >= 0 && page_id < p.num_pages;
       if (live && !inside) report_bad_index(p.dev_status);
       mask = __ballot_sync(0xffffffffu, live && inside) & 0xffffu;
       const int slot = j - page_of(p, j) * p.page;
-      const int64_t ko = live && inside ? page_id * p.skp + slot * p.sks + k_head : 0;
-      const int64_t vo = live && inside ? page_id * p.svp + slot * p.svs + v_head : 0;
+      const int64_t ko = live && inside ? page_id * p.skp + slot * p.sks + hkv * p.skh : 0;
+      const int64_t vo = live && inside ? page_id * p.svp + slot * p.svs + hkv * p.svh : 0;
       if (mask) {
 #pragma unroll
         for (int i = 0; i < SUB / ROWS_AT_ONCE; ++i) {
           const int row = i * ROWS_AT_ONCE + row_in;
           const int64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
           const bool get = chunk_there && (mask >> row & 1);
-          const uint32_t dst = stage + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);
+          const uint32_t dst = to + place_of(row, chunk);
           cp_async16(dst, get ? K + kr + chunk * 8 : K, get ? 16 : 0);
           cp_async16(dst + V_OFF, get ? V + vr + chunk * 8 : V, get ? 16 : 0);
         }
@@ -173,38 +167,52 @@ struct Producer {
         at.next_unit(p);
         enter_unit(p);
       }
-    } else if (!WHOLE_PAGE || at.t - first == 32) {
+    } else if (!TMA || at.t - first == 32) {
       look_up(p);
     }
     return mask;
   }
 };
 
-template <typename T, int DP, int NT, bool WHOLE_PAGE>
-__global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma_kernel(const PagedParams p) {
+template <typename T, int DP, int NT, bool TMA>
+__global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm)
+paged_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedParams p) {
   constexpr int STAGES = Shape<DP, NT>::stages, STAGE_BYTES = Shape<DP, NT>::stage_bytes, V_OFF = STAGE_BYTES / 2;
   constexpr int KSTEPS = DP / 16;
-  extern __shared__ __align__(128) char smem[];
+  extern __shared__ char smem_raw[];
+  __shared__ uint64_t full[4][STAGES];
+  __shared__ int gave_up;
   __shared__ uint32_t there[4][STAGES];  // which of a stage's 16 keys exist
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   grid_dependency_trigger();
+  if (TMA && threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    for (int w = 0; w < 4; ++w)
+      for (int s = 0; s < STAGES; ++s) mbar_init(&full[w][s], 1);
+    gave_up = 0;
+    fence_barrier_init();
+  }
   int64_t lo, hi;
   TileCursor at;
-  if (!find_stretch<THREADS>(p, lo, hi, at)) return;
+  if (!find_stretch<THREADS>(p, lo, hi, at)) return;  // (its barriers follow the mbarriers' set-up)
 
-  const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE_BYTES;
-  char* const ring_ptr = smem + warp * STAGES * STAGE_BYTES;
-  const T* const K = static_cast<const T*>(p.k);
-  const T* const V = static_cast<const T*>(p.v);
-  Producer<T, DP, WHOLE_PAGE> producer;
+  char* const ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u) + warp * STAGES * STAGE_BYTES;
+  Producer<T, DP, TMA> producer;
   producer.begin(p, at, hi - lo);
   auto fetch = [&](int stage) {
     if (producer.left > 0) {
-      const uint32_t mask = producer.fetch(p, K, V, ring + stage * STAGE_BYTES);
+      const uint32_t mask = producer.fetch(p, &tm_k, &tm_v, ring + stage * STAGE_BYTES, &full[warp][stage]);
       if (lane == 0) there[warp][stage] = mask;
     }
-    cp_async_commit();
+    if (!TMA) cp_async_commit();
+  };
+  uint32_t parity = 0;  // of the next wait on each stage
+  auto wait_for = [&](int stage) {
+    const bool ok = mbar_wait(&full[warp][stage], parity >> stage & 1, &gave_up, p.dev_status, DEV_TIMEOUT_PAGED);
+    parity ^= 1u << stage;
+    return __all_sync(0xffffffffu, ok) != 0;
   };
 
   // ---- a unit: lane r knows query row r of it, the fragments of Q are loaded
@@ -267,12 +275,32 @@ __global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma
   clear();
   int stage = 0;
   for (int64_t left = hi - lo; left > 0; --left) {
-    cp_async_wait<STAGES - 1>();
+    if (!TMA) cp_async_wait<STAGES - 1>();
     __syncwarp();
     const uint32_t mask = there[warp][stage];
+    char* const here = ring + stage * STAGE_BYTES;
+    bool wrote = false;  // with plain stores, into a stage that the TMA writes next
     if (mask) {
-      const uint32_t base = ring + stage * STAGE_BYTES;
+      const uint32_t base = smem_u32(here);
       const int key0 = at.t * TILE;
+      if constexpr (TMA) {
+        if (!wait_for(stage)) {  // the copies never came: leave, but let those of the other stages come in
+          for (int s = 1; s < STAGES; ++s) {
+            const int other = (stage + s) % STAGES;
+            int late = 0;
+            if (left > s && there[warp][other]) mbar_wait_limit(&full[warp][other], parity >> other & 1, &late, nullptr, 0, LH_WAIT_TIMEOUT_NS);
+          }
+          return;
+        }
+        if (mask != 0xffffu) {  // rows behind the last key hold anything: of V, zeros
+          wrote = true;
+          for (int i = lane; i < SUB * (DP / 8); i += 32) {
+            const int row = i / (DP / 8), chunk = i % (DP / 8);
+            if (!(mask >> row & 1)) *reinterpret_cast<uint4*>(here + V_OFF + place_of(row, chunk)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          __syncwarp();
+        }
+      }
       float s[NT][4], s2[NT][4];  // even and odd steps: two chains of half the length
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -281,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
         uint32_t a[4];
-        ldmatrix4(a, base + krow * (DP * 2) + (((k * 2 + kchunk) ^ (krow & 7)) << 4));
+        ldmatrix4(a, base + place_of(krow, k * 2 + kchunk));
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma16816<T>(k & 1 ? s2[n] : s[n], a, qf[n][k][0], qf[n][k][1]);
       }
@@ -340,12 +368,12 @@ __global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma
         bool odd = false;
         for (int r = max(0, at.len - p.Sq + 1 - key0); r < SUB && (mask >> r & 1); ++r)
           for (int c = lane; c < DP; c += 32) {
-            const float v = bits_to_f32<T>(reinterpret_cast<const unsigned short*>(ring_ptr + stage * STAGE_BYTES + V_OFF + r * (DP * 2))[c]);
+            const float v = bits_to_f32<T>(*reinterpret_cast<const unsigned short*>(here + V_OFF + place_of(r, c >> 3) + (c & 7) * 2));
             odd |= !(fabsf(v) < INFINITY);
           }
         if (__any_sync(0xffffffffu, odd)) {
+          wrote = true;
           for (int r = max(0, at.len - p.Sq + 1 - key0); r < SUB; ++r) {
-            char* const row = ring_ptr + stage * STAGE_BYTES + V_OFF + r * (DP * 2);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint32_t two = __shfl_sync(0xffffffffu, r < 8 ? pf[n][0] : pf[n][1], (r & 7) * 4 + t4);
@@ -354,13 +382,13 @@ __global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma
               for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                  const float v = bits_to_f32<T>(*reinterpret_cast<const unsigned short*>(row + (((k * 2 + i) ^ (r & 7)) << 4) + g * 2));
+                  const float v = bits_to_f32<T>(*reinterpret_cast<const unsigned short*>(here + V_OFF + place_of(r, k * 2 + i) + g * 2));
                   if (p0 != 0.f) acc[n][k][i * 2] = fmaf(p0, v, acc[n][k][i * 2]);
                   if (p1 != 0.f) acc[n][k][i * 2 + 1] = fmaf(p1, v, acc[n][k][i * 2 + 1]);
                 }
             }
             __syncwarp();
-            for (int c = lane; c < DP / 2; c += 32) reinterpret_cast<uint32_t*>(row)[c] = 0u;
+            for (int c = lane; c < DP / 8; c += 32) *reinterpret_cast<uint4*>(here + V_OFF + place_of(r, c)) = make_uint4(0u, 0u, 0u, 0u);
           }
           __syncwarp();
         }
@@ -373,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
         uint32_t a[4];
-        ldmatrix4_trans(a, base + V_OFF + vrow * (DP * 2) + (((k * 2 + vchunk) ^ (vrow & 7)) << 4));
+        ldmatrix4_trans(a, base + V_OFF + place_of(vrow, k * 2 + vchunk));
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma16816<T>(acc[n][k], a, pf[n][0], pf[n][1]);
       }
@@ -383,7 +411,8 @@ __global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma
       // ---- the warp leaves the unit. The stage just used takes two n tiles of results as rows of f32;
       // dimensions are swizzled by the row so that neither side meets in a bank. The next unit's
       // Q is on its way meanwhile.
-      float* const buf = reinterpret_cast<float*>(ring_ptr + stage * STAGE_BYTES);
+      float* const buf = reinterpret_cast<float*>(here);
+      wrote = true;
       const int64_t slot = partial_slot<THREADS>(t0, at.t, at.tiles);
       const int64_t rows_at = slot < 0 ? o_row : (slot * p.part_rows + lane) * p.Dp;
       const int n_done = nrows;
@@ -436,6 +465,10 @@ __global__ void __launch_bounds__(THREADS, Shape<DP, NT>::ctas_per_sm) paged_mma
       }
       clear();
     }
+    if (TMA && wrote) {
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
     fetch(stage);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
@@ -448,13 +481,32 @@ int n_tiles_for(int rows, int D) {
   return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
 }
 
-typedef void (*PagedKernel)(const PagedParams);
+// A pool as a tensor (dimension, row of a page, head, page) for the TMA; false where that cannot be: tiles
+// across pages, an empty pool, strides that repeat elements.
+bool encode_pool(lh_ctx* ctx, CUtensorMap* map, int dtype, const void* base, const PagedParams& p, int64_t slot, int64_t head, int64_t page) {
+  if (p.page % TILE || p.num_pages < 1) return false;
+  const uint64_t dims[4] = {static_cast<uint64_t>(p.D), static_cast<uint64_t>(p.page), static_cast<uint64_t>(p.Hkv), static_cast<uint64_t>(p.num_pages)};
+  uint64_t strides[3];
+  const int64_t elements[3] = {slot, head, page};
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i + 1] > 1 && (elements[i] <= 0 || elements[i] >= int64_t(1) << 38)) return false;
+    strides[i] = dims[i + 1] > 1 ? static_cast<uint64_t>(elements[i]) * 2 : 16;
+  }
+  const uint32_t box[4] = {64, TILE, 1, 1};
+  return encode_tensor_map(ctx, map, dtype, 4, const_cast<void*>(base), dims, strides, box, 1) == LH_OK;
+}
+
 template <typename T, int DP, int NT>
 int launch(lh_ctx* ctx, const PagedParams& p, int ctas) {
-  constexpr int smem = THREADS / 32 * Shape<DP, NT>::stages * Shape<DP, NT>::stage_bytes;
-  PagedKernel kernel = p.page % SUB == 0 ? paged_mma_kernel<T, DP, NT, true> : paged_mma_kernel<T, DP, NT, false>;
+  constexpr int smem = THREADS / 32 * Shape<DP, NT>::stages * Shape<DP, NT>::stage_bytes + 1024;  // the swizzle wants 1024-byte boundaries
+  const int dtype = std::is_same<T, __half>::value ? LH_F16 : LH_BF16;
+  CUtensorMap k, v;
+  memset(&k, 0, sizeof(k));
+  memset(&v, 0, sizeof(v));
+  const bool tma = encode_pool(ctx, &k, dtype, p.k, p, p.sks, p.skh, p.skp) && encode_pool(ctx, &v, dtype, p.v, p, p.svs, p.svh, p.svp);
+  auto* kernel = tma ? paged_mma_kernel<T, DP, NT, true> : paged_mma_kernel<T, DP, NT, false>;
   LH_CUDA_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kernel<<<static_cast<unsigned>(ctas), THREADS, smem, ctx->stream>>>(p);
+  kernel<<<static_cast<unsigned>(ctas), THREADS, smem, ctx->stream>>>(k, v, p);
   LH_CHECK_LAUNCH(ctx, "paged_mma_kernel");
   return LH_OK;
 }

@@ -27,6 +27,7 @@ enum DeviceError : int {
   DEV_TIMEOUT_CORRECTION = 105,
   DEV_TIMEOUT_PEER = 106,      // a flag another rank writes did not arrive
   DEV_TIMEOUT_SELFTEST = 107,  // the wait the self-test lets run out on purpose
+  DEV_TIMEOUT_PAGED = 108,     // a tile of the paged cache did not arrive
   DEV_BAD_INDEX = 201,         // a page, slot or length operand points outside its table; the access was skipped
 };
 
