@@ -252,9 +252,9 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
   __shared__ uint32_t there[S::warps][S::stages];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_dependency_trigger();
-  int64_t lo, hi;
   TileCursor at;
-  if (!find_stretch<THREADS>(p, lo, hi, at)) return;
+  int64_t left = find_stretch<THREADS>(p, at);
+  if (left == 0) return;
   float* const ring = ring_mem + warp * S::template warp_floats<R>();
   float* const qs = ring + S::stages * S::stage_floats;
   float* const ps = qs + R * S::q_pitch;
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
 
   Fetch f;
   f.at = at;
-  f.left = hi - lo;
+  f.left = left;
   f.look_up(p, lane & 15);
   auto fetch = [&](int stage) {
     if (f.left <= 0) return;
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
   int seen[R];
   int t0 = at.t, stage = 0;
   bool fresh = true;
-  for (int64_t left = hi - lo; left > 0; --left) {
+  for (; left > 0; --left) {
     const int hkv = at.u / p.row_groups, row0 = (at.u % p.row_groups) * R;
     const int nrows = min(R, p.rows - row0);
     if (fresh) {
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) paged_join_kernel(const Pa
     if (here.x >= 0 && here.z > 0) {  // a stretch that begins inside its unit
       const int64_t total = *p.total;
       const int64_t n = total < stretches ? total : stretches;
-      const int64_t begin = stretch_begin(total, n, i) - here.z;
+      const int64_t begin = stretch_begin(total, n, i) - here.z;  // the unit's first tile
       if (stretch_begin(total, n, i - 1) <= begin) {  // no earlier border lies in this unit
         const int64_t end = begin + here.w;
         w.c0 = i - 1;
@@ -816,6 +816,9 @@ extern "C" int lh_b200_paged_attention(lh_ctx_t* ctx, const lh_memref_t* o, cons
   const bool mma = paged_mma_supported(k_pages, v_pages);
   p.unit_rows = mma ? paged_mma_unit_rows(p.rows, p.D) : simt_unit_rows(p.rows);
   p.part_rows = std::min(p.rows, p.unit_rows);
+  // A unit's Q and epilogue against a tile, measured inside the kernels: 2000 clocks to 1000 with eight
+  // rows, 3800 to 1300 with more; the FFMA kernel's tiles take as long as its epilogue.
+  p.unit_cost = !mma ? 1 : p.unit_rows == 8 ? 2 : 3;
   const int stretches = mma ? paged_mma_stretches(ctx, p.rows, p.D) : simt_stretches(ctx, p.D);
   p.o_vec = p.D % 4 == 0 && aligned_view(o, 4);
   p.q_pairs = dtype_size(q->dtype) == 2 && aligned_view(q, 2);

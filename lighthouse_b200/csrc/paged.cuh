@@ -1,10 +1,13 @@
 // Attention of new tokens over a paged key-value cache: what its kernels share. The keys of a
 // sequence are cut into tiles of 16; all tiles of a call form one line (sequence, then unit, then
 // tile; a unit is a kv head and a group of its query rows), and every WARP takes an equal stretch
-// of that line, with loads, online softmax and results of its own. The lengths live on the
-// device, so each CTA works out its warps' stretches itself: a call needs no knowledge of them on
-// the host, replays as a graph while sequences grow, and a ragged batch is balanced to within one
-// tile. Where a stretch ends inside a unit, the warp leaves a partial result to the join kernel.
+// of that line, with loads, online softmax and results of its own. A unit costs its warp some tiles' time
+// besides its tiles (Q, the epilogue), so the line counts that too: a unit takes unit_cost places and
+// then one per tile, and a stretch that would begin within the former begins with the unit. The
+// lengths live on the device, so each CTA works out its warps' stretches itself: a call needs
+// no knowledge of them on the host, replays as a graph while sequences grow, and a ragged batch
+// is balanced. Where a stretch ends inside a unit, the warp leaves a partial result to the join
+// kernel.
 #pragma once
 #include "common.cuh"
 #include "epilogue.cuh"
@@ -27,11 +30,12 @@ struct PagedParams {
   int page, page_shift;   // page_shift < 0: the page size is no power of two
   int max_keys;           // table columns x page size
   int rows, unit_rows, row_groups;  // query rows of a kv head (tokens x group), rows of a unit, units of a kv head
+  int unit_cost;          // places on the line that a unit takes besides its tiles
   int o_dtype, o_vec;     // o_vec: four elements of a row of o can be stored at once
   int q_pairs;            // two 16-bit elements of a row of q can be loaded at once
   float scale_log2;       // softmax scale x log2(e): scores are kept as powers of two
   // workspace
-  int64_t* total;         // tiles of the whole call
+  int64_t* total;         // length of the line
   int4* first;            // per stretch: (sequence, unit, tile) it starts at and the unit's tiles; x < 0: it has none
   float2* ml;             // per partial row: running maximum and sum
   float* part;            // per partial row: Dp floats, not yet divided by the sum
@@ -42,14 +46,17 @@ struct PagedParams {
 constexpr int TILE = 16;  // keys of a tile
 constexpr int JOIN_WARPS = 8;
 
-// Stretch i of n is tiles [total * i / n, total * (i + 1) / n); none is empty because n <= total.
+// Stretch i of n is places [total * i / n, total * (i + 1) / n) of the line; n <= total.
 // (n is some thousands at most, so 32-bit division serves all but the longest calls in a quarter of the time.)
 __host__ __device__ __forceinline__ int64_t stretch_begin(int64_t total, int64_t n, int64_t i) {
   const int64_t x = total * i;
   return x < 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(n)) : x / n;
 }
-// The stretch that has tile x: the last i with total * i / n < x + 1.
-__host__ __device__ __forceinline__ int64_t stretch_owner(int64_t total, int64_t n, int64_t x) { return ((x + 1) * n - 1) / total; }
+// The stretch that has place x: the last i with total * i / n < x + 1.
+__host__ __device__ __forceinline__ int64_t stretch_owner(int64_t total, int64_t n, int64_t x) {
+  const int64_t y = (x + 1) * n - 1;
+  return y < 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(y) / static_cast<uint32_t>(total)) : y / total;
+}
 
 __device__ __forceinline__ int paged_length(const PagedParams& p, int b) {
   const int len = p.lengths[b * p.slen];
@@ -62,13 +69,14 @@ __device__ __forceinline__ int page_of(const PagedParams& p, int j) { return p.p
 // A position on the line of tiles.
 struct TileCursor {
   int b, u, t, tiles, len;
+  // `within`: places from the sequence's first on.
   __device__ __forceinline__ void seek(const PagedParams& p, int b_, int64_t within) {
     b = b_;
     len = paged_length(p, b);
     tiles = paged_tiles(len);
-    // a sequence has at most 2^27 tiles, and its units are as many as fit 31 bits: only the longest need 64
-    u = within < 0x7fffffff ? static_cast<int>(static_cast<uint32_t>(within) / static_cast<uint32_t>(tiles)) : static_cast<int>(within / tiles);
-    t = static_cast<int>(within - static_cast<int64_t>(u) * tiles);
+    const int unit = tiles + p.unit_cost;
+    u = within < 0x7fffffff ? static_cast<int>(static_cast<uint32_t>(within) / static_cast<uint32_t>(unit)) : static_cast<int>(within / unit);
+    t = max(0, static_cast<int>(within - static_cast<int64_t>(u) * unit) - p.unit_cost);
   }
   // Only called while tiles of this warp's stretch remain, so the next sequence exists.
   __device__ __forceinline__ void next_unit(const PagedParams& p) {
@@ -83,71 +91,93 @@ struct TileCursor {
   }
 };
 
-// Each warp gets its stretch [lo, hi) and where it starts; false for warps without one. Prefix sum over
-// the sequences: each thread adds up a run of them, the block scans the runs. All threads call it.
+// Each warp learns how many tiles its stretch has and where it starts; 0 for warps without any. Prefix
+// sums over the sequences: each thread adds up a run of them, the block scans the runs. All
+// threads call it.
 template <int NT>
-__device__ __forceinline__ bool find_stretch(const PagedParams& p, int64_t& lo, int64_t& hi, TileCursor& at) {
+__device__ __forceinline__ int64_t find_stretch(const PagedParams& p, TileCursor& at) {
   constexpr int W = NT / 32;
-  __shared__ int64_t warp_sum[W];
-  __shared__ int64_t start_base[W];
-  __shared__ int start_b[W];
+  __shared__ int64_t warp_places[W], warp_tiles[W];
+  __shared__ int64_t start_places[W + 1], start_tiles[W + 1];  // of the sequence that each border lies in: places from its first on, tiles before it
+  __shared__ int start_b[W + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int units = p.Hkv * p.row_groups;
   const int run = (p.B + NT - 1) / NT;
   const int64_t first = static_cast<int64_t>(tid) * run;  // B can be near 2^31
   const int b0 = first < p.B ? static_cast<int>(first) : p.B;
   const int b1 = first + run < p.B ? static_cast<int>(first + run) : p.B;
-  int64_t mine = 0;
+  auto tiles_of = [&](int b) { return paged_tiles(paged_length(p, b)); };
+  auto places_of = [&](int tiles) { return tiles ? static_cast<int64_t>(tiles + p.unit_cost) * units : 0; };
+  int64_t my_places = 0, my_tiles = 0;
   for (int b = b0; b < b1; ++b) {
     const int raw = p.lengths[b * p.slen];
     if (blockIdx.x == 0 && (raw < 0 || raw > p.max_keys)) report_bad_index(p.dev_status);
-    mine += static_cast<int64_t>(paged_tiles(paged_length(p, b))) * units;
+    const int tiles = tiles_of(b);
+    my_places += places_of(tiles);
+    my_tiles += static_cast<int64_t>(tiles) * units;
   }
-  int64_t incl = mine;
+  int64_t places = my_places, tiles_incl = my_tiles;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += up;
+    const int64_t up = __shfl_up_sync(0xffffffffu, places, d), up_t = __shfl_up_sync(0xffffffffu, tiles_incl, d);
+    if (lane >= d) {
+      places += up;
+      tiles_incl += up_t;
+    }
   }
-  if (lane == 31) warp_sum[warp] = incl;
+  if (lane == 31) {
+    warp_places[warp] = places;
+    warp_tiles[warp] = tiles_incl;
+  }
   __syncthreads();
-  int64_t before = 0, total = 0;
+  int64_t total = 0, all_tiles = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
+    if (w < warp) {
+      places += warp_places[w];
+      tiles_incl += warp_tiles[w];
+    }
+    total += warp_places[w];
+    all_tiles += warp_tiles[w];
   }
   const int64_t stretches = static_cast<int64_t>(gridDim.x) * W;
   const int64_t n = total < stretches ? total : stretches;
   if (blockIdx.x == 0 && tid == 0) *p.total = total;
-  const int64_t base = before + incl - mine;
-  for (int w = 0; w < W; ++w) {
+  const int64_t base = places - my_places;
+  for (int w = 0; w <= W; ++w) {  // the CTA's borders: where each warp's stretch begins, and the last one's ends
     const int64_t s = static_cast<int64_t>(blockIdx.x) * W + w;
     if (s >= n) break;
     const int64_t begin = stretch_begin(total, n, s);
-    if (begin < base || begin >= base + mine) continue;
-    int64_t at_base = base;
+    if (begin < base || begin >= places) continue;
+    int64_t at_place = base, at_tile = tiles_incl - my_tiles;
     for (int b = b0; b < b1; ++b) {
-      const int64_t here = static_cast<int64_t>(paged_tiles(paged_length(p, b))) * units;
-      if (begin < at_base + here) {
+      const int tiles = tiles_of(b);
+      const int64_t here = places_of(tiles);
+      if (begin < at_place + here) {
         start_b[w] = b;
-        start_base[w] = at_base;
+        start_places[w] = begin - at_place;
+        start_tiles[w] = at_tile;
         break;
       }
-      at_base += here;
+      at_place += here;
+      at_tile += static_cast<int64_t>(tiles) * units;
     }
   }
   __syncthreads();
   const int64_t s = static_cast<int64_t>(blockIdx.x) * W + warp;
-  if (s >= n) {
-    if (lane == 0) p.first[s] = make_int4(-1, 0, 0, 0);
-    return false;
+  int64_t left = 0;
+  if (s < n) {
+    int64_t end = all_tiles;
+    if (s + 1 < n) {
+      TileCursor to;
+      to.seek(p, start_b[warp + 1], start_places[warp + 1]);
+      end = start_tiles[warp + 1] + static_cast<int64_t>(to.u) * to.tiles + to.t;
+    }
+    at.seek(p, start_b[warp], start_places[warp]);
+    left = end - (start_tiles[warp] + static_cast<int64_t>(at.u) * at.tiles + at.t);
   }
-  lo = stretch_begin(total, n, s);
-  hi = stretch_begin(total, n, s + 1);
-  at.seek(p, start_b[warp], lo - start_base[warp]);
-  if (lane == 0) p.first[s] = make_int4(at.b, at.u, at.t, at.tiles);
-  return true;
+  if (lane == 0) p.first[s] = left ? make_int4(at.b, at.u, at.t, at.tiles) : make_int4(-1, 0, 0, 0);
+  return left;
 }
 
 // Where a warp's part of a unit (tiles t0 .. t1 of `tiles`) goes: -1 when it is the whole unit, else

@@ -194,13 +194,13 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     gave_up = 0;
     fence_barrier_init();
   }
-  int64_t lo, hi;
   TileCursor at;
-  if (!find_stretch<THREADS>(p, lo, hi, at)) return;  // (its barriers follow the mbarriers' set-up)
+  int64_t left = find_stretch<THREADS>(p, at);
+  if (left == 0) return;  // (its barriers follow the mbarriers' set-up)
 
   char* const ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u) + warp * STAGES * STAGE_BYTES;
   Producer<T, DP, TMA> producer;
-  producer.begin(p, at, hi - lo);
+  producer.begin(p, at, left);
   auto fetch = [&](int stage) {
     if (producer.left > 0) {
       const uint32_t mask = producer.fetch(p, &tm_k, &tm_v, ring + stage * STAGE_BYTES, &full[warp][stage]);
@@ -274,7 +274,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   };
   clear();
   int stage = 0;
-  for (int64_t left = hi - lo; left > 0; --left) {
+  for (; left > 0; --left) {
     if (!TMA) cp_async_wait<STAGES - 1>();
     __syncwarp();
     const uint32_t mask = there[warp][stage];
