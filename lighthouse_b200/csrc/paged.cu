@@ -225,8 +225,8 @@ constexpr int SIMT_ROWS = 8;
 
 template <int DP>
 struct SimtShape {
-  static constexpr int warps = DP == 256 ? 2 : 4;
-  static constexpr int stages = 3;
+  static constexpr int warps = DP == 256 ? 3 : 6;
+  static constexpr int stages = 2;
   static constexpr int stage_floats = 2 * TILE * DP;  // K and V rows of 16 keys
   static constexpr int ctas_per_sm = DP == 64 ? 2 : 1;
   static constexpr int q_pitch = DP + 8;  // the second half of a row is 4 floats further: no bank in common
@@ -324,11 +324,20 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
       fresh = false;
       t0 = at.t;
       __syncwarp();
-      for (int i = lane; i < R * DP; i += 32) {
-        const int r = i / DP, d = i % DP;
-        float x = 0.f;
-        if (r < nrows && d < p.D) x = to_f32(static_cast<const T*>(p.q)[at.b * p.sqb + row_head(p, hkv, row0 + r) * p.sqh + row_token(p, row0 + r) * p.sqs + d]) * p.scale_log2;
-        qs[r * S::q_pitch + d + (d >= DP / 2 ? 4 : 0)] = x;
+      constexpr int TOGETHER = R * DP / 32 < 16 ? R * DP / 32 : 16;  // loads on their way at a time
+#pragma unroll 1
+      for (int i0 = lane; i0 < R * DP; i0 += 32 * TOGETHER) {
+        float x[TOGETHER];
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) {
+          const int r = (i0 + k * 32) / DP, d = (i0 + k * 32) % DP;
+          x[k] = r < nrows && d < p.D ? to_f32(static_cast<const T*>(p.q)[at.b * p.sqb + row_head(p, hkv, row0 + r) * p.sqh + row_token(p, row0 + r) * p.sqs + d]) * p.scale_log2 : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) {
+          const int r = (i0 + k * 32) / DP, d = (i0 + k * 32) % DP;
+          qs[r * S::q_pitch + d + (d >= DP / 2 ? 4 : 0)] = x[k];
+        }
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
