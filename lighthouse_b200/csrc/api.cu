@@ -840,6 +840,10 @@ static int run_ops(lh_module* m, void* const* arg_ptrs) {
         // other operators that need some (sized when the module was created)
         lh_memref_t ws;
         if (!o[6] && o[1] && o[2]) {
+          if (ctx->side_selected) {  // the scratch may be in use on the main stream
+            rc = set_error(ctx, LH_ERR_UNSUPPORTED, "paged_attention on the side stream needs a workspace operand");
+            break;
+          }
           size_t need = 0;
           rc = lh_b200_paged_attention_workspace(ctx, o[1], o[2], &need);
           if (!rc) rc = ensure_scratch(ctx, need);

@@ -358,6 +358,99 @@ def build_llama_plan(cfg: LlamaConfig, rank: int = 0, tp: int = 1, name: str = "
     return p
 
 
+@dataclass(frozen=True)
+class PagedCache:
+    """The key-value cache of one layer: ``pages`` pages of ``page_size`` rows, of which a
+    sequence may have ``columns`` (its row of the page table)."""
+
+    pages: int
+    columns: int
+    page_size: int = 64
+
+    def shape(self, cfg: LlamaConfig, tp: int = 1) -> tuple[int, int, int, int]:
+        return (self.pages, self.page_size, cfg.n_kv_heads // tp, cfg.head_dim)
+
+
+def build_llama_decode_plan(cfg: LlamaConfig, cache: PagedCache, vocab: int, rank: int = 0, tp: int = 1, name: str = "llama_decode") -> Plan:
+    """One step of generation for ``cfg.batch`` sequences with ``cfg.seq`` new tokens each (one
+    when decoding, more for a piece of the prompt or for proposed tokens): embedding, the
+    decoder stack over a paged key-value cache, the logits after each sequence's last token, and
+    the token drawn from them.
+
+    Args: ``tokens (batch) i32, logprobs (batch) f32, logits (batch, vocab) f32`` (results), then
+    ``ids (tokens) i32, slots (tokens) i64, positions (tokens) i32, page_table (batch, columns) i32,
+    lengths (batch) i32`` (with the new tokens), ``uniform, temperature (batch) f32, top_k (batch)
+    i32, top_p, min_p (batch) f32, [k_pages, v_pages] * n_layer, wte (vocab, dim),
+    [attention_norm, wqkv, wo, ffn_norm, w13, w2] * n_layer, norm, lm_head (vocab, dim)``.
+
+    A sequence with fewer new tokens than ``cfg.seq`` has them at the end of its row, behind
+    padding whose slots are -1; one with none has a length of 0. The drawn ``tokens`` may be the
+    next step's ``ids`` as they are. With ``tp`` > 1 every rank has its heads' part of the cache,
+    embedding and head are whole on each, and all ranks draw the same tokens.
+    """
+    check_tp(cfg, tp)
+    if vocab < 1 or cache.pages < 1 or cache.columns < 1 or cache.page_size < 1:
+        raise ValueError("a decoding plan needs a vocabulary and a cache of at least one page")
+    d, t, hd, n = cfg.dim, cfg.tokens, cfg.head_dim, cfg.batch
+    hq, hkv, fl = cfg.n_heads // tp, cfg.n_kv_heads // tp, cfg.ffn // tp
+    ql, kl = hq * hd, hkv * hd
+    width = ql + 2 * kl
+    args = [
+        ArgSpec((n,), "i32", "tokens"), ArgSpec((n,), "f32", "logprobs"), ArgSpec((n, vocab), "f32", "logits"),
+        ArgSpec((t,), "i32", "ids"), ArgSpec((t,), "i64", "slots"), ArgSpec((t,), "i32", "positions"),
+        ArgSpec((n, cache.columns), "i32", "page_table"), ArgSpec((n,), "i32", "lengths"),
+        ArgSpec((n,), "f32", "uniform"), ArgSpec((n,), "f32", "temperature"), ArgSpec((n,), "i32", "top_k"),
+        ArgSpec((n,), "f32", "top_p"), ArgSpec((n,), "f32", "min_p"),
+    ]
+    first_page = len(args)
+    for li in range(cfg.n_layer):
+        args += [ArgSpec(cache.shape(cfg, tp), "bf16", f"l{li}.{k}") for k in ("k_pages", "v_pages")]
+    args.append(ArgSpec((vocab, d), "bf16", "wte"))
+    first_weight = len(args)
+    per_layer = [((d,), "bf16"), ((width, d), "bf16"), ((d, ql), "bf16"), ((d,), "bf16"), ((2 * fl, d), "bf16"), ((d, fl), "bf16")]
+    for li in range(cfg.n_layer):
+        args += [ArgSpec(s, dt, f"l{li}.{k}") for (s, dt), k in zip(per_layer, LLAMA_LAYER_KEYS)]
+    args += [ArgSpec((d,), "bf16", "norm"), ArgSpec((vocab, d), "bf16", "lm_head")]
+    p = Plan(name, args)
+    tokens, logprobs, logits, ids, slots, positions, page_table, lengths, uniform, temperature, top_k, top_p, min_p = (p.arg(i) for i in range(first_page))
+    h = p.temp((t, d), "bf16")      # residual stream
+    hn = p.temp((t, d), "bf16")
+    qkv = p.temp((t, width), "bf16")
+    att = p.temp((t, ql), "bf16")
+    ff = p.temp((t, fl), "bf16")
+
+    def heads(view2d: PView, col0: int, nheads: int) -> PView:  # (tokens, heads, head_dim)
+        v = view2d.slice(1, col0, nheads * hd)
+        return PView(v.slot, (t, nheads, hd), (v.strides[0], hd, 1), v.dtype, v.offset)
+
+    def bhsd(view2d: PView) -> PView:
+        return PView(view2d.slot, (n, hq, cfg.seq, hd), (cfg.seq * view2d.strides[0], hd, view2d.strides[0], 1), view2d.dtype, view2d.offset)
+
+    first = rank == 0
+    p.embedding(h, ids, p.arg(first_weight - 1))
+    for li in range(cfg.n_layer):
+        a = {k: p.arg(first_weight + li * len(LLAMA_LAYER_KEYS) + i) for i, k in enumerate(LLAMA_LAYER_KEYS)}
+        k_pages, v_pages = p.arg(first_page + 2 * li), p.arg(first_page + 2 * li + 1)
+        p.rmsnorm(hn, h, a["attention_norm"], cfg.eps)
+        p.gemm(qkv, hn, a["wqkv"].t())
+        p.paged_append(heads(qkv, 0, hq), heads(qkv, ql, hkv), heads(qkv, ql + kl, hkv), k_pages, v_pages, slots, positions, cfg.theta)
+        p.paged_attention(bhsd(att), bhsd(qkv), k_pages, v_pages, page_table, lengths, 1.0 / math.sqrt(hd))
+        p.gemm(h, att, a["wo"].t(), residual=h if first else None)
+        if tp > 1:
+            p.allreduce(h)
+        p.rmsnorm(hn, h, a["ffn_norm"], cfg.eps)
+        p.gemm(ff, hn, a["w13"].t(), swiglu=True)
+        p.gemm(h, ff, a["w2"].t(), residual=h if first else None)
+        if tp > 1:
+            p.allreduce(h)
+    last = PView(h.slot, (n, d), (cfg.seq * d, 1), h.dtype, h.offset + (cfg.seq - 1) * d)  # each sequence's last token
+    out = hn.slice(0, 0, n)
+    p.rmsnorm(out, last, p.arg(len(args) - 2), cfg.eps)
+    p.gemm(logits, out, p.arg(len(args) - 1).t())
+    p.sample(tokens, logits, uniform, temperature, top_k, top_p, min_p, logprobs)
+    return p
+
+
 class _SideChain:
     """Bookkeeping for plans that overlap collectives with compute: each micro-batch's
     contracting GEMM on the main stream is followed, on the side stream, by reduce-scatter ->
@@ -526,6 +619,13 @@ def flatten_nanogpt_args(w: dict) -> list:
     for lw in w["layers"]:
         out += [lw[k] for k in GPT_LAYER_KEYS]
     return out + [w["gf_g"], w["gf_b"], w["lmw"], w["lmb"]]
+
+
+def llama_decode_caches(cfg: LlamaConfig, cache: PagedCache, tp: int = 1, device="cuda") -> list:
+    """``[k_pages, v_pages] * n_layer`` for ``build_llama_decode_plan``, empty."""
+    import torch
+
+    return [torch.zeros(cache.shape(cfg, tp), dtype=torch.bfloat16, device=device) for _ in range(2 * cfg.n_layer)]
 
 
 def flatten_llama_args(w: dict) -> list:
