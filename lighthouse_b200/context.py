@@ -198,6 +198,8 @@ class CudaContext:
     # seven descriptors through ctypes would take 20.
     def _entry(self, name: str):
         """(call, address) of an entry point, looked up once."""
+        if not self.handle:
+            raise ValueError(f"{name}: the context is closed")
         found = self._entries.get(name)
         if found is None:
             found = self._entries[name] = (N.binding().call, N.address(name))
@@ -255,11 +257,13 @@ class CudaContext:
 
     def _new_workspace(self, nbytes: int) -> N.MemRef:
         torch = _torch()
-        t = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+        stream, capturing = self._stream_info  # as _kept_workspace left them
+        # in the stream's own order: memory that another stream freed may still be written by what that one has queued
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream.value or 0, device=self.device)):
+            t = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
         # none is given back while the context lives: work still queued, or a captured graph, may use it
         self._workspaces_held.append(t)
         ws = self._bytes(t)
-        stream, capturing = self._stream_info  # as _kept_workspace left them
         if not capturing.value:
             self._workspaces[stream.value] = ws
         return ws

@@ -646,6 +646,8 @@ bool aligned_view(const lh_memref_t* m, int elems) {
   return true;
 }
 
+bool aligned_to_type(const lh_memref_t* m) { return reinterpret_cast<uintptr_t>(data_ptr(m)) % dtype_size(m->dtype) == 0; }
+
 bool float_type(int dt) { return dt == LH_F32 || dt == LH_BF16 || dt == LH_F16; }
 
 // A view that is written: no element of it may be two elements.
@@ -689,6 +691,8 @@ int check_attention(lh_ctx* ctx, const lh_memref_t* o, const lh_memref_t* q, con
   if (k->shape[3] != q->shape[3] || q->shape[3] < 1) return set_error(ctx, LH_ERR_INVALID, "paged_attention: head sizes of q and the pages differ, or are zero");
   if (k->shape[2] < 1 || q->shape[1] % k->shape[2]) return set_error(ctx, LH_ERR_INVALID, "paged_attention: %lld query heads are not a multiple of %lld kv heads", (long long)q->shape[1], (long long)k->shape[2]);
   if (k->shape[1] < 1) return set_error(ctx, LH_ERR_INVALID, "paged_attention: page size must be at least 1");
+  for (const lh_memref_t* m : {o, q, k, v, table, lengths})
+    if (!aligned_to_type(m)) return set_error(ctx, LH_ERR_INVALID, "paged_attention: an operand is not aligned to its type");
   if (table->dtype != LH_I32 || lengths->dtype != LH_I32) return set_error(ctx, LH_ERR_INVALID, "paged_attention: page_table and lengths are i32");
   if (q->dtype != k->dtype || q->dtype != v->dtype) return set_error(ctx, LH_ERR_INVALID, "paged_attention: q and the pages must have one type");
   if (!float_type(q->dtype) || !float_type(o->dtype)) return set_error(ctx, LH_ERR_UNSUPPORTED, "paged_attention: f32, bf16 or f16 operands");
@@ -737,6 +741,8 @@ extern "C" int lh_b200_paged_append(lh_ctx_t* ctx, const lh_memref_t* q, const l
     if (m && D > 1 && m->strides[m->rank - 1] != 1) return set_error(ctx, LH_ERR_UNSUPPORTED, "paged_append: the head dimension must have unit stride");
   for (const lh_memref_t* m : {q, k_pages, v_pages})
     if (m && overlaps_itself(m)) return set_error(ctx, LH_ERR_INVALID, "paged_append: a written operand overlaps itself (zero stride)");
+  for (const lh_memref_t* m : {q, k, v, k_pages, v_pages, slots, positions})
+    if (m && !aligned_to_type(m)) return set_error(ctx, LH_ERR_INVALID, "paged_append: an operand is not aligned to its type");
   const int64_t Hq = q ? q->shape[1] : 0;
   if ((Hq + 2 * k->shape[1]) * D > 0x7fffffffll) return set_error(ctx, LH_ERR_UNSUPPORTED, "paged_append: a token's rows are too long");
   if (T == 0) return LH_OK;

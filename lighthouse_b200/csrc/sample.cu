@@ -822,13 +822,14 @@ extern "C" int lh_b200_sample(lh_ctx_t* ctx, const lh_memref_t* tokens, const lh
   if (v > MAX_VOCAB) return set_error(ctx, LH_ERR_UNSUPPORTED, "sample: a vocabulary of %lld is above %lld", (long long)v, (long long)MAX_VOCAB);
   if (logits->dtype != LH_F32 && logits->dtype != LH_BF16 && logits->dtype != LH_F16) return set_error(ctx, LH_ERR_UNSUPPORTED, "sample: f32, bf16 or f16 logits");
   if (v > 1 && logits->strides[1] != 1) return set_error(ctx, LH_ERR_UNSUPPORTED, "sample: a row of logits must have unit stride");
-  if (reinterpret_cast<uintptr_t>(data_ptr(logits)) % dtype_size(logits->dtype)) return set_error(ctx, LH_ERR_INVALID, "sample: logits are not aligned to their type");
   for (const lh_memref_t* m : {tokens, logprobs, uniform, temperature, top_k, top_p, min_p})
     if (m && !vector_of(m, n)) return set_error(ctx, LH_ERR_INVALID, "sample: tokens, logprobs, uniform and the settings have one entry per row");
   for (const lh_memref_t* m : {logprobs, uniform, temperature, top_p, min_p})
     if (m && m->dtype != LH_F32) return set_error(ctx, LH_ERR_INVALID, "sample: logprobs, uniform, temperature, top_p and min_p are f32");
   for (const lh_memref_t* m : {tokens, top_k})
     if (m && m->dtype != LH_I32 && m->dtype != LH_I64) return set_error(ctx, LH_ERR_INVALID, "sample: tokens and top_k are i32 or i64");
+  for (const lh_memref_t* m : {tokens, logprobs, logits, uniform, temperature, top_k, top_p, min_p})
+    if (m && reinterpret_cast<uintptr_t>(data_ptr(m)) % dtype_size(m->dtype)) return set_error(ctx, LH_ERR_INVALID, "sample: an operand is not aligned to its type");
   for (const lh_memref_t* m : {tokens, logprobs})
     if (m && n > 1 && m->strides[0] == 0) return set_error(ctx, LH_ERR_INVALID, "sample: a written operand overlaps itself (zero stride)");
   if (n == 0) return LH_OK;

@@ -537,3 +537,71 @@ def test_sample_and_append_in_a_graph(native_lib):
             want, _ = R.sample(host(x), un, top_p=[np.float32(0.9)] * 5)
             assert (t.cpu().numpy() == want).all()
             assert torch.equal(kp.view(64, 2, 64)[torch.from_numpy(sn).cuda().long()], k)
+
+
+def test_a_kept_workspace_is_not_memory_that_another_stream_has_yet_to_write(own_stream_ctx):
+    c = own_stream_ctx
+    q = torch.zeros(1, 4, 1, 64, device="cuda", dtype=torch.bfloat16)
+    k = torch.ones(2, 16, 1, 64, device="cuda", dtype=torch.bfloat16)
+    tab, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.full((1,), 16, dtype=torch.int32, device="cuda")
+    o = torch.empty_like(q)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    freed = torch.empty(c.paged_attention_workspace(q, k), dtype=torch.uint8, device="cuda")
+    at = freed.data_ptr()
+    del freed  # torch's current stream may have it again at once, the context's may not
+    c.paged_attention(o, q, k, k, tab, lens, 0.1)
+    c.sync()
+    assert c._workspaces_held[-1].data_ptr() != at
+    assert (o == 1).all()
+
+
+def test_operands_off_their_types_boundaries_and_a_closed_context(native_lib, own_stream_ctx):
+    c = own_stream_ctx
+    raw = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+
+    def odd(code, *shape):
+        strides = N.contiguous_strides(shape)
+        return N.memref(raw.data_ptr() + 1, shape, strides, code)
+
+    q = torch.zeros(1, 2, 1, 8, device="cuda")
+    k = torch.zeros(1, 16, 2, 8, device="cuda")
+    i = torch.zeros(1, dtype=torch.int32, device="cuda")
+    good = dict(o=q.clone(), q=q, k_pages=k, v_pages=k, page_table=i[None], lengths=i, scale=1.0)
+    for name, bad in (("o", odd(N.LH_F32, 1, 2, 1, 8)), ("q", odd(N.LH_F32, 1, 2, 1, 8)), ("k_pages", odd(N.LH_F32, 1, 16, 2, 8)), ("v_pages", odd(N.LH_F32, 1, 16, 2, 8)), ("page_table", odd(N.LH_I32, 1, 1)), ("lengths", odd(N.LH_I32, 1))):
+        with pytest.raises(ValueError, match="aligned"):
+            c.paged_attention(**{**good, name: bad})
+    good = dict(q=None, k=q[0, :, 0][None], v=q[0, :, 0][None], k_pages=k, v_pages=k.clone(), slots=i, positions=i)
+    for name, bad in (("k", odd(N.LH_F32, 1, 2, 8)), ("v_pages", odd(N.LH_F32, 1, 16, 2, 8)), ("slots", odd(N.LH_I64, 1)), ("positions", odd(N.LH_I32, 1))):
+        with pytest.raises(ValueError, match="aligned"):
+            c.paged_append(**{**good, name: bad})
+    x, u = torch.zeros(1, 10, device="cuda"), torch.zeros(1, device="cuda")
+    for bad in (dict(tokens=odd(N.LH_I32, 1)), dict(logits=odd(N.LH_F32, 1, 10)), dict(uniform=odd(N.LH_F32, 1)), dict(top_k=odd(N.LH_I32, 1)), dict(logprobs=odd(N.LH_F32, 1))):
+        with pytest.raises(ValueError, match="aligned"):
+            c.sample(**{**dict(tokens=i, logits=x, uniform=u), **bad})
+    from lighthouse_b200.context import CudaContext
+
+    closed = CudaContext(0)
+    closed.close()
+    with pytest.raises(ValueError, match="closed"):
+        closed.sample(i, x, u)
+    with pytest.raises(ValueError, match="closed"):
+        closed.paged_append(None, q[0], q[0], k, k, i, i)
+    with pytest.raises(ValueError, match="closed"):
+        closed.paged_attention(q, q, k, k, i[None], i, 1.0)
+
+
+def test_the_result_may_take_the_querys_place(ctx):
+    """o and q one tensor: a unit's rows of q are read by the warps of that unit alone, and written after."""
+    rng = np.random.default_rng(31)
+    lengths = [5, 700, 0, 4000, 33]
+    k, v, table = cache_of(rng, lengths, 16, 2, 64, "bf16")
+    q = randn(rng, 5, 16, 2, 64, dtype="bf16")
+    tab, lens = torch.from_numpy(table).cuda(), torch.tensor(lengths, dtype=torch.int32).cuda()
+    apart, both = torch.empty_like(q), q.clone()
+    ctx.paged_attention(apart, q, k, v, tab, lens, 0.125)
+    for _ in range(3):
+        both.copy_(q)
+        ctx.paged_attention(both, both, k, v, tab, lens, 0.125)
+        ctx.sync()
+        assert torch.equal(both, apart)
