@@ -492,8 +492,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) paged_join_kernel(const Pa
   JoinWork w = {0, 0, 0, 0};
   if (i > 0 && i < stretches) {
     const int4 here = p.first[i];  // the unit's tiles with it: nothing to look up in turn
+    const int64_t total = *p.total;
     if (here.x >= 0 && here.z > 0) {  // a stretch that begins inside its unit
-      const int64_t total = *p.total;
       const int64_t n = total < stretches ? total : stretches;
       const int64_t begin = stretch_begin(total, n, i) - here.z;  // the unit's first tile
       if (stretch_begin(total, n, i - 1) <= begin) {  // no earlier border lies in this unit
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) paged_join_kernel(const Pa
       }
     }
   }
-  __syncthreads();
+  if (!__syncthreads_or(w.parts > ALONE)) return;
   for (int q = 0; q < JOIN_WARPS; ++q) {
     w = work[q];
     if (w.parts <= ALONE) continue;
