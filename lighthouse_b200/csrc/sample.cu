@@ -60,7 +60,8 @@ constexpr float BINS_PER_OCTAVE = 93.f;  // the last bin starts 44 octaves below
 constexpr int DIGIT_BITS = 11;
 constexpr int DIGITS = 1 << DIGIT_BITS;
 constexpr int LIST = 1024;
-constexpr int TABLE = 16;
+constexpr int TABLE = 64;
+constexpr int COPIES = 16;  // of the table: the half of a warp that a 64-bit load serves at a time finds a bank for each lane
 
 __device__ __forceinline__ float as_f32(float x) { return x; }
 __device__ __forceinline__ float as_f32(__half x) { return __half2float(x); }
@@ -90,8 +91,9 @@ struct Tally {
 struct Weighing {
   float top, half_top;
   float bin_scale;       // bins per two units of logit
-  double top64, scale;   // row maximum; 16 log2(e) / T
-  const double* table;   // 2^(42 + i / 16), this lane's copy: 32 apart, no two lanes meet in a bank
+  float lowest;          // what is not above it (NaN is not) weighs nothing
+  double top64, scale;   // row maximum; 64 log2(e) / T
+  const double* table;   // 2^(42 + i / 64), this lane's copy
 
   // Distance from the maximum in bins. Falls with x; 0 for the maximum, BINS - 1 for NaN, -inf and
   // whatever weighs nothing. (Halves: the difference of two finite logits stays finite.)
@@ -99,25 +101,27 @@ struct Weighing {
   // Rounding towards zero by adding 2^23 keeps the conversion off the slow units.
   __device__ __forceinline__ int bin_of(float x) const { return __float_as_int(__fadd_rd(place_of(x), 8388608.f)) & (BINS - 1); }
 
-  // 2^42 times the weight, not yet a whole number.
-  // 2^t = 2^(j / 16) (1 + (e^(f ln2 / 16) - 1)), 16 t = j + f, |f| <= 1/2: the series' sixth term
-  // and on are below 2^-42.
+  // 2^42 times the weight, not yet a whole number, of a logit above `lowest`.
+  // 2^t = 2^(j / 64) (1 + (e^(f ln2 / 64) - 1)), 64 t = j + f, |f| <= 1/2: the series' fifth term
+  // and on are below 2^-44.
   __device__ __forceinline__ double of(float x) const {
-    double y = (static_cast<double>(x) - top64) * scale;
-    const double lowest = -(WEIGHT_BITS + 1.0) * TABLE;  // a half: no weight
-    y = y > lowest ? y : lowest;                          // also for NaN, and -inf * 0
-    const double magic = 6755399441055744.0;              // 1.5 * 2^52: the sum's low bits are the nearest whole number
-    const double z = y + magic;
+    const double d = static_cast<double>(x) - top64;
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double z = fma(d, scale, magic);
     const int j = __double2loint(z);
-    const double f = y - (z - magic);
-    constexpr double a1 = 0.69314718055994530942 / TABLE, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4, a5 = a4 * a1 / 5;
-    const double s = f * fma(f, fma(f, fma(f, fma(f, a5, a4), a3), a2), a1);
+    const double f = fma(d, scale, magic - z);
+    constexpr double a1 = 0.69314718055994530942 / TABLE, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4;
+    const double s = f * fma(f, fma(f, fma(f, a4, a3), a2), a1);
     const int low = j & (TABLE - 1);
-    const double base = table[low * 32];
+    const double base = table[low * COPIES];
     const double scaled = __hiloint2double(__double2hiint(base) + (j - low) * ((1 << 20) / TABLE), __double2loint(base));
     return fma(scaled, s, scaled);
   }
-  __device__ __forceinline__ u64 whole(float x) const { return Tally().add(of(x)).value(); }
+  __device__ __forceinline__ bool counts(float x) const { return x > lowest; }
+  __device__ __forceinline__ u64 whole(float x) const {
+    const u64 w = Tally().add(of(x)).value();  // (whatever it is at logits that do not count)
+    return w & (counts(x) ? ~0ull : 0ull);
+  }
 };
 
 template <typename V>
@@ -151,12 +155,12 @@ struct Answer {
 static_assert(sizeof(Answer) % sizeof(u64) == 0, "copied in words");
 
 struct Shared {
-  double table[TABLE * 32];
+  double table[TABLE * COPIES];
   u64 digits[DIGITS];      // sums of a digit; or, as 32-bit words, of the bins
   // The CTA's candidates, and in the lead everybody's (`mass` by place in the list). Between uses of
   // the list the lead keeps the cluster's sums of bins or digits here.
   u64 list[LIST], mass[LIST];
-  u64 kept[MAX_RUNS], middle[MAX_RUNS], rest[MAX_RUNS];  // lead: weights before, in and behind the candidates, per run
+  u64 kept[MAX_RUNS], middle[MAX_RUNS], all[MAX_RUNS];  // lead: weights before the candidates, of them and of everything, per run
   u64 red[WARPS];
   Answer answer;
   float tops[MAX_CLUSTER];
@@ -465,21 +469,23 @@ struct Sampler {
   }
   __device__ __forceinline__ u64 weight_of(u64 order) const { return weigh.whole(value_of(static_cast<uint32_t>(order >> INDEX_BITS))); }
 
-  // Lead: sorts the list and finds the place at which the running count or weight reaches `want`.
+  // Lead: sorts the list and finds the place at which the running count or weight reaches `want`;
+  // returns the list's whole count or weight, which `want` may be beyond.
   template <bool BY_MASS>
-  __device__ void rank_list(int n, u64 want) {
+  __device__ u64 rank_list(int n, u64 want) {
+    u64 all = n;
     sort_list(n);
     if (!BY_MASS) {
       if (threadIdx.x == 0) sh.answer.border = sh.list[want - 1];
     } else {
       const int c = 2 * threadIdx.x;
       const u64 w0 = c < n ? weight_of(sh.list[c]) : 0, w1 = c + 1 < n ? weight_of(sh.list[c + 1]) : 0;
-      u64 all;
       const u64 before = block_before(w0 + w1, sh.red, all);
       if (before < want && want <= before + w0) sh.answer.border = sh.list[c];
       else if (before + w0 < want && want <= before + w0 + w1) sh.answer.border = sh.list[c + 1];
     }
     __syncthreads();
+    return all;
   }
 
   // Lead: the list holds everything that top-k may keep. The rest of the row's work is done on it.
@@ -617,7 +623,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) sample_kernel(const Samp
   // ---- the maximum (fmaxf passes NaN over)
   float top = -INFINITY;
   me.each([&](float x, int) { top = fmaxf(top, x); });
-  for (int i = tid; i < TABLE * 32; i += THREADS) sh.table[i] = exp2(static_cast<double>(i / 32) / TABLE) * WEIGHT_ONE;
+  {
+    constexpr int MINE = TABLE * COPIES / THREADS;  // copies of one value, by each thread
+    const double value = exp2(static_cast<double>(tid * MINE / COPIES) / TABLE) * WEIGHT_ONE;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) sh.table[tid * MINE + i] = value;
+  }
   me.clear_bins();
   if (tid == 0) sh.listed = 0;
   const float temperature = p.temperature ? p.temperature[r * p.st] : 1.f;
@@ -688,7 +699,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) sample_kernel(const Samp
   weigh.bin_scale = fminf(2.f * BINS_PER_OCTAVE * 1.44269504f / temperature, 3e38f);
   weigh.top64 = static_cast<double>(top);
   weigh.scale = TABLE * 1.4426950408889634073599 / static_cast<double>(temperature);
-  weigh.table = sh.table + lane;
+  // 2^-43 of the largest, rounded down: a whole weight of zero there, and above it at least 2^-43. (Below
+  // the maximum also where that many units are lost in its last place.)
+  weigh.lowest = fminf(__double2float_rd(weigh.top64 - (WEIGHT_BITS + 1) * 0.69314718055994530942 * static_cast<double>(temperature)), nextafterf(top, -INFINITY));
+  weigh.table = sh.table + lane % COPIES;
   const u64 least = min_p > 0.f ? __double2ull_ru(fmin(static_cast<double>(min_p), 1.0) * static_cast<double>(WEIGHT_ONE)) : 0;
   u64 border = 0;
   bool have_runs = false;  // the answer already says which run the draw lies in
@@ -729,39 +743,44 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) sample_kernel(const Samp
     me.template find_bins<true>(0, static_cast<double>(top_p), border);
     do {
       const float from = sh.answer.from, to = sh.answer.to;
-      Tally all, before, middle;
+      Tally all, before;
       me.each([&](float x, int i) {
         if (border && order_of(x, i) < border) return;
         const double w = weigh.of(x);
-        all.add(w);
+        if (weigh.counts(x)) all.add(w);
         if (x > from) before.add(w);
-        else if (x > to) {
-          middle.add(w);
-          me.collect(order_of(x, i));
-        }
+        else if (x > to) me.collect(order_of(x, i));
       });
-      const u64 a = warp_total(before.value()), m = warp_total(middle.value()), z = warp_total(all.value());
+      const u64 a = warp_total(before.value()), z = warp_total(all.value());
       if (lane == 0) {
         me.lead.kept[run] = a;
-        me.lead.middle[run] = m;
-        me.lead.rest[run] = z - a - m;
+        me.lead.all[run] = z;
       }
       const int n = me.gather();
+      if (n > LIST) {  // their weight, which else the ranked list gives
+        u64 m = 0;
+        me.each([&](float x, int i) {
+          if (x > to && x <= from && !(border && order_of(x, i) < border)) m += weigh.whole(x);
+        });
+        m = warp_total(m);
+        if (lane == 0) me.lead.middle[run] = m;
+        cluster.sync();
+      }
       if (me.is_lead()) {
-        // three sums in one: they are few enough for every warp to add them up itself
-        u64 a = 0, m = 0, z = 0;
+        // the sums are few enough for every warp to add them up itself
+        u64 a = 0, z = 0, m = 0;
         for (int c = lane; c < me.runs(); c += 32) {
           a += sh.kept[c];
-          m += sh.middle[c];
-          z += sh.rest[c];
+          z += sh.all[c];
+          if (n > LIST) m += sh.middle[c];
         }
         a = warp_total(a);
-        m = warp_total(m);
         z = warp_total(z);
-        const u64 need = share_of(top_p, a + m + z);
+        m = warp_total(m);
+        const u64 need = share_of(top_p, z);
+        if (a < need && n <= LIST) m = me.template rank_list<true>(n, need - a);
         const bool right = a < need && need <= a + m;
         if (right && n <= LIST) {
-          me.template rank_list<true>(n, need - a);
           const u64 found = sh.answer.border;
           for (int c = tid; c < n; c += THREADS)
             if (sh.list[c] >= found) atomicAdd(&sh.kept[me.run_of(index_of(sh.list[c]))], me.weight_of(sh.list[c]));
@@ -793,7 +812,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) sample_kernel(const Samp
       me.each([&](float x, int i) { mine += kept_weight(x, i); });
     } else {
       Tally all;
-      me.each([&](float x, int) { all.add(weigh.of(x)); });
+      me.each([&](float x, int) {
+        const double w = weigh.of(x);
+        if (weigh.counts(x)) all.add(w);
+      });
       mine = all.value();
     }
     mine = warp_total(mine);
