@@ -219,8 +219,10 @@ AppendKernel append_vec_for(int q_dtype, int c_dtype) {
 // f32 with four query rows to a kv head it needs 512 FFMA and about 250 shared-memory wavefronts
 // per 16 keys of D = 128 (16 KB), half of what an SM has time for while those bytes arrive.
 // A warp fetches 16 keys at a time into a ring of f32 rows (cp.async; or, ASYNC false, loads and
-// conversions of single elements). Scores: a lane has a key and half of its dimensions. P V: a lane
-// has four dimensions (of 64 only half the lanes' worth: the halves take alternate keys).
+// conversions of single elements). Scores: a lane has four keys and an eighth of their dimensions, so
+// that a load of Q serves four keys and one of K all rows; the eighths are then added up in halving
+// steps, after which a lane has one key and half of the rows. P V: a lane has four dimensions (of
+// 64 only half the lanes' worth: the halves take alternate keys).
 constexpr int SIMT_ROWS = 8;
 
 template <int DP>
@@ -229,7 +231,7 @@ struct SimtShape {
   static constexpr int stages = 2;
   static constexpr int stage_floats = 2 * TILE * DP;  // K and V rows of 16 keys
   static constexpr int ctas_per_sm = DP == 64 ? 2 : 1;
-  static constexpr int q_pitch = DP + 8;  // the second half of a row is 4 floats further: no bank in common
+  static constexpr int q_pitch = DP;
   template <int R>
   static constexpr int warp_floats() { return stages * stage_floats + R * q_pitch + TILE * R; }
   template <int R>
@@ -246,7 +248,8 @@ __device__ __forceinline__ float to_f32(T x) {
 template <typename T, int DP, int R, bool ASYNC>
 __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas_per_sm) paged_simt_kernel(const PagedParams p) {
   using S = SimtShape<DP>;
-  constexpr int THREADS = S::warps * 32, CHUNKS = DP / 4, HALF = CHUNKS / 2;
+  constexpr int THREADS = S::warps * 32, CHUNKS = DP / 4;
+  constexpr int RH = R / 2;  // rows of which a lane has the scores
   constexpr int NV = DP == 256 ? 2 : 1, AT_ONCE = DP == 64 ? 2 : 1;  // P V: vectors of a lane, keys taken at once
   extern __shared__ __align__(16) float ring_mem[];
   __shared__ uint32_t there[S::warps][S::stages];
@@ -311,10 +314,12 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
     cp_async_commit();
   }
 
-  const int key = lane & 15, half = lane >> 4;
+  const int eighth = lane & 7, key4 = (lane >> 3) * 4;      // of the products
+  const int key = key4 + (eighth >> 1), rows0 = (lane & 1) * RH;  // of the scores
+  const int half = lane >> 4;
   const int my_chunk = DP == 64 ? lane & 15 : lane;  // P V
-  float m[R], l[R], acc[R][NV * 4];
-  int seen[R];
+  float m[RH], l[RH], acc[R][NV * 4];
+  int seen[RH];
   int t0 = at.t, stage = 0;
   bool fresh = true;
   for (; left > 0; --left) {
@@ -336,14 +341,17 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
 #pragma unroll
         for (int k = 0; k < TOGETHER; ++k) {
           const int r = (i0 + k * 32) / DP, d = (i0 + k * 32) % DP;
-          qs[r * S::q_pitch + d + (d >= DP / 2 ? 4 : 0)] = x[k];
+          qs[r * S::q_pitch + d] = x[k];
         }
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int r = 0; r < RH; ++r) {
         m[r] = -INFINITY;
         l[r] = 0.f;
-        seen[r] = r < nrows ? at.len - p.Sq + 1 + row_token(p, row0 + r) : 0;  // keys that the row may attend to
+        seen[r] = rows0 + r < nrows ? at.len - p.Sq + 1 + row_token(p, row0 + rows0 + r) : 0;  // keys that the row may attend to
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
 #pragma unroll
         for (int i = 0; i < NV * 4; ++i) acc[r][i] = 0.f;
       }
@@ -355,47 +363,74 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
       const float* const kt = ring + stage * S::stage_floats;
       const float* const vt = kt + TILE * DP;
       const int key0 = at.t * TILE;
-      float s[R];
+      float part[R][4];
 #pragma unroll
-      for (int r = 0; r < R; ++r) s[r] = 0.f;
-#pragma unroll 8
-      for (int c = 0; c < HALF; ++c) {
-        const float4 kv = *reinterpret_cast<const float4*>(kt + key * DP + (((half * HALF + c) ^ (key & 7)) << 2));
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[r][k] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CHUNKS / 8; ++c) {
+        float4 kv[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) kv[k] = *reinterpret_cast<const float4*>(kt + (key4 + k) * DP + (((c * 8 + eighth) ^ ((key4 + k) & 7)) << 2));
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float4 qv = *reinterpret_cast<const float4*>(qs + r * S::q_pitch + half * (DP / 2 + 4) + c * 4);
-          s[r] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[r]))));
+          const float4 qv = *reinterpret_cast<const float4*>(qs + r * S::q_pitch + (c * 8 + eighth) * 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) part[r][k] = fmaf(qv.x, kv[k].x, fmaf(qv.y, kv[k].y, fmaf(qv.z, kv[k].z, fmaf(qv.w, kv[k].w, part[r][k]))));
         }
+      }
+      // Each step gives half of what is left to the lane across and adds what comes back: keys 2 and 3 against 0
+      // and 1, then the odd key, then the second half of the rows.
+      float two[R][2], one[R], s[RH];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float give = lane & 4 ? part[r][k] : part[r][k + 2];
+          two[r][k] = (lane & 4 ? part[r][k + 2] : part[r][k]) + __shfl_xor_sync(0xffffffffu, give, 4);
+        }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float give = lane & 2 ? two[r][0] : two[r][1];
+        one[r] = (lane & 2 ? two[r][1] : two[r][0]) + __shfl_xor_sync(0xffffffffu, give, 2);
+      }
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+        const float give = lane & 1 ? one[r] : one[r + RH];
+        s[r] = (lane & 1 ? one[r + RH] : one[r]) + __shfl_xor_sync(0xffffffffu, give, 1);
       }
       // keys that only the later of several new tokens may see: masked rows must not meet their V
       const bool partial = key0 + TILE > at.len - p.Sq + 1;
       bool grows = false;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        s[r] += __shfl_xor_sync(0xffffffffu, s[r], 16);
+      for (int r = 0; r < RH; ++r) {
         if (!(mask >> key & 1) || key0 + key >= seen[r]) s[r] = -INFINITY;
         grows |= s[r] > m[r];
       }
       // the running maximum is only brought up to date when some key passes it
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int r = 0; r < RH; ++r) {
           float top = s[r];
 #pragma unroll
-          for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          for (int d = 2; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           top = fmaxf(top, m[r]);
-          const float alpha = top == -INFINITY ? 1.f : exp2f(m[r] - top);
+          const float alpha = top == -INFINITY ? 1.f : exp2f(m[r] - top), others = __shfl_xor_sync(0xffffffffu, alpha, 1);
           m[r] = top;
           l[r] *= alpha;
 #pragma unroll
-          for (int i = 0; i < NV * 4; ++i) acc[r][i] *= alpha;
+          for (int i = 0; i < NV * 4; ++i) {
+            acc[r][i] *= lane & 1 ? others : alpha;
+            acc[r + RH][i] *= lane & 1 ? alpha : others;
+          }
         }
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int r = 0; r < RH; ++r) {
         const float e = exp2_safe(s[r], m[r]);
         l[r] += e;
-        if (half == 0) ps[key * R + r] = e;
+        ps[key * R + rows0 + r] = e;
       }
       __syncwarp();
 #pragma unroll 4
@@ -422,18 +457,27 @@ __global__ void __launch_bounds__(SimtShape<DP>::warps * 32, SimtShape<DP>::ctas
     if (++at.t == at.tiles || left == 1) {
       // ---- the warp leaves the unit
       const int64_t slot = partial_slot<THREADS>(t0, at.t, at.tiles);
+      float m_of[R], l_of[R];
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+#pragma unroll
+        for (int d = 2; d < 32; d <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+        const float m_other = __shfl_xor_sync(0xffffffffu, m[r], 1), l_other = __shfl_xor_sync(0xffffffffu, l[r], 1);
+        m_of[r] = lane & 1 ? m_other : m[r];
+        m_of[r + RH] = lane & 1 ? m[r] : m_other;
+        l_of[r] = lane & 1 ? l_other : l[r];
+        l_of[r + RH] = lane & 1 ? l[r] : l_other;
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-#pragma unroll
-        for (int d = 8; d; d >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);  // the two halves hold the same keys
         if (AT_ONCE == 2) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[r][i] += __shfl_xor_sync(0xffffffffu, acc[r][i], 16);
         }
         if (r >= nrows) continue;
-        const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];  // a row that sees no key has no weight: zeros
+        const float inv = l_of[r] == 0.f ? 0.f : 1.f / l_of[r];  // a row that sees no key has no weight: zeros
         const int64_t out = at.b * p.sob + row_head(p, hkv, row0 + r) * p.soh + row_token(p, row0 + r) * p.sos;
-        if (slot >= 0 && lane == 0) p.ml[slot * p.part_rows + r] = make_float2(m[r], l[r]);
+        if (slot >= 0 && lane == 0) p.ml[slot * p.part_rows + r] = make_float2(m_of[r], l_of[r]);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int d = (my_chunk + i * 32) * 4;
