@@ -217,6 +217,24 @@ def test_entry_points_without_a_context(native_lib):
     assert native_lib.lh_b200_sample(none, none, none, none, none, none, none, none, none) == -1
 
 
+def test_binding_refuses_what_it_cannot_read(native_lib):
+    call, sample, append = N.binding().call, N.address("lh_b200_sample"), N.address("lh_b200_paged_append")
+    x = torch.zeros(2, 8)
+    some = N.memref(256, (2, 8), (8, 1), N.LH_F32)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        call(sample, None, 0, None, x, None, x, x, None, None, None, None)
+    with pytest.raises(TypeError, match="not list"):
+        call(sample, None, 0, None, [1], None, some, some, None, None, None, None)
+    for wrong in ((sample, None, 0, None, some), (append, None, 0, 1.0, some), (append, None, 0, None) + (some,) * 7, (sample,)):
+        with pytest.raises(TypeError, match="operands"):
+            call(*wrong)
+    with pytest.raises(TypeError):
+        call(append, None, 0, "theta", *(some,) * 7)
+    # read, passed on, and refused there: no context
+    assert call(sample, None, 0, None, some, None, some, some, None, None, None, None) == -1
+    assert call(append, None, 0, 0.5, None, *(some,) * 6) == -1
+
+
 def test_oracle_of_bad_pages_and_lengths():
     rng = np.random.default_rng(0)
     k, v = rng.standard_normal((2, 3, 2, 1, 4))

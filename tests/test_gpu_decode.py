@@ -605,3 +605,87 @@ def test_the_result_may_take_the_querys_place(ctx):
         ctx.paged_attention(both, both, k, v, tab, lens, 0.125)
         ctx.sync()
         assert torch.equal(both, apart)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 8), ("f16", 16), ("bf16", 24), ("bf16", 136), ("f16", 200), ("bf16", 248), ("f32", 4), ("f32", 1), ("f32", 252)])
+@pytest.mark.parametrize("page", [16, 48])
+def test_attention_smallest_and_odd_head_sizes(ctx, dtype, d, page):
+    rng = np.random.default_rng(d + page)
+    lengths = [1, 47, 48, 49, 300]
+    k, v, table = cache_of(rng, lengths, page, 2, d, dtype)
+    q = randn(rng, 5, 6, 1, d, dtype=dtype)
+    check_attention(ctx, torch.empty_like(q), q, k, v, table, lengths, d**-0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("tokens,hq,hkv,d", [(200, 8, 2, 64), (3, 100, 1, 128), (1, 64, 1, 64), (70, 2, 2, 256), (1, 33, 1, 40)])
+def test_attention_many_rows_to_a_kv_head(ctx, dtype, tokens, hq, hkv, d):
+    """A piece of a prompt, or many heads on one: units of more rows than one pass takes."""
+    rng = np.random.default_rng(tokens + hq)
+    lengths = [tokens, tokens + 130, max(1, tokens - 5), 0]
+    k, v, table = cache_of(rng, lengths, 16, hkv, d, dtype)
+    q = randn(rng, 4, hq, tokens, d, dtype=dtype)
+    check_attention(ctx, torch.empty_like(q), q, k, v, table, lengths, d**-0.5)
+
+
+def test_attention_thousands_of_sequences(ctx):
+    rng = np.random.default_rng(8)
+    lengths = rng.integers(0, 20, 5000).tolist()
+    k, v, table = cache_of(rng, lengths, 8, 1, 32, "bf16")
+    q = randn(rng, 5000, 2, 1, 32, dtype="bf16")
+    check_attention(ctx, torch.empty_like(q), q, k, v, table, lengths, 0.2)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_over_an_empty_pool_or_table(ctx, dtype):
+    """Nothing to read: lengths of zero give zeros, others are reported and give zeros."""
+    q = torch.ones(2, 4, 1, 64, dtype=TYPES[dtype], device="cuda")
+    some, none = torch.ones(3, 16, 2, 64, dtype=TYPES[dtype], device="cuda"), torch.ones(0, 16, 2, 64, dtype=TYPES[dtype], device="cuda")
+    columns = lambda n: torch.zeros(2, n, dtype=torch.int32, device="cuda")
+    for pool, table in ((some, columns(0)), (none, columns(2)), (none, columns(0))):
+        for lengths, bad in (([0, 0], False), ([5, 0], True)):
+            o = torch.full_like(q, 7.0)
+            ctx.paged_attention(o, q, pool, pool, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), 0.125)
+            if bad:
+                with pytest.raises(N.LighthouseCudaError, match="outside its table"):
+                    ctx.sync()
+            else:
+                ctx.sync()
+            assert not o.any()
+    k = torch.ones(2, 2, 64, dtype=TYPES[dtype], device="cuda")
+    at = torch.zeros(2, dtype=torch.int32, device="cuda")
+    ctx.paged_append(None, k, k, none, none, at - 1, at)  # all padding
+    ctx.sync()
+    ctx.paged_append(None, k, k, none, none, at, at)
+    with pytest.raises(N.LighthouseCudaError, match="outside its table"):
+        ctx.sync()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sample_top_p_borders_among_many_equal_logits(ctx, dtype):
+    """More candidates than the lead ranks, with and without top-k before; borders at their first and last."""
+    rng = np.random.default_rng(6)
+    rows, vocab = 9, 30000
+    x = torch.full((rows, vocab), -3.0, dtype=TYPES[dtype], device="cuda")
+    x[:, ::7] = 1.0
+    x[:, 5] = 2.0
+    p = np.array([1e-6, 1e-4, 0.05, 0.3, 0.7, 0.95, 0.9999, 0.99999, 1.0], np.float32)
+    for temperature in (0.5, 1.0, 4.0):
+        for more in ({}, dict(top_k=[20000] * rows), dict(top_k=[2000] * rows), dict(min_p=[0.1] * rows)):
+            check_sample(ctx, x, rng.random(rows, dtype=np.float32), temperature=[temperature] * rows, top_p=p, **more)
+
+
+def test_on_torchs_default_stream(native_lib):
+    """A context made where nobody chose a stream: the legacy default one, workspace included."""
+    from lighthouse_b200.context import CudaContext
+
+    rng = np.random.default_rng(41)
+    k, v, table = cache_of(rng, [100, 300], 16, 2, 64, "bf16")
+    q = randn(rng, 2, 4, 1, 64, dtype="bf16")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.default_stream()), CudaContext(0, use_torch_stream=True) as c:
+        o = torch.empty_like(q)
+        for _ in range(2):
+            check_attention(c, o, q, k, v, table, [100, 300], 0.125)
+        check_sample(c, randn(rng, 3, 1000), rng.random(3, dtype=np.float32), top_p=[0.9] * 3)
+        torch.cuda.synchronize()
