@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32, 4) paged_join_kernel(const Pa
     const int4 here = p.first[i];  // the unit's tiles with it: nothing to look up in turn
     const int64_t total = *p.total;
     if (here.x >= 0 && here.z > 0) {  // a stretch that begins inside its unit
-      const int64_t n = total < stretches ? total : stretches;
+      const int64_t n = stretch_count(total, stretches);
       const int64_t begin = stretch_begin(total, n, i) - here.z;  // the unit's first tile
       if (stretch_begin(total, n, i - 1) <= begin) {  // no earlier border lies in this unit
         const int64_t end = begin + here.w;
