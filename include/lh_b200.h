@@ -293,7 +293,7 @@ int lh_b200_paged_append(lh_ctx_t* ctx, const lh_memref_t* q, const lh_memref_t*
  * fixes the order of every sum, so a call repeats bit for bit.
  * workspace: contiguous, 256-byte aligned, at least lh_b200_paged_attention_workspace bytes
  * (LH_ERR_NOMEM below that); calls that can overlap on the GPU need one each. In a module the
- * operand may be absent: the context's scratch is used.
+ * operand may be absent: the context's scratch is used, on the main stream only.
  */
 int lh_b200_paged_attention(lh_ctx_t* ctx, const lh_memref_t* o, const lh_memref_t* q, const lh_memref_t* k_pages,
                             const lh_memref_t* v_pages, const lh_memref_t* page_table, const lh_memref_t* lengths,
